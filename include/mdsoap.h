@@ -38,7 +38,9 @@ typedef enum {
     MDSOAP_INTERNAL = 6
 } mdsoap_status;
 
-typedef enum { MDSOAP_FLOAT32 = 0, MDSOAP_FLOAT64 = 1 } mdsoap_dtype;
+/* Element types.  SOAP rows are float32 or float64; the readout operators at
+ * the end of this header take float32, bfloat16 and float16. */
+typedef enum { MDSOAP_FLOAT32 = 0, MDSOAP_FLOAT64 = 1, MDSOAP_BFLOAT16 = 2, MDSOAP_FLOAT16 = 3 } mdsoap_dtype;
 
 typedef enum { MDSOAP_AVERAGE_OFF = 0, MDSOAP_AVERAGE_INNER = 1, MDSOAP_AVERAGE_OUTER = 2 } mdsoap_average;
 
@@ -386,6 +388,108 @@ int64_t mdsoap_local_feature_count(const mdsoap_local_params* params);
  * (cpp/cuda/src/backend.cu:590-624). */
 int mdsoap_local_compute(const mdsoap_local_params* params, const mdsoap_batch* batch, double* out,
                          int32_t device);
+
+/* ------------------------------------------------------------------------
+ * Readout operators: what a network trained on descriptor rows needs between
+ * the rows and its answers (no counterpart in the reference, which stops at
+ * the rows).  All pointers are device memory on `device`; matrices are row
+ * major with unit column stride and a row pitch ("stride") in elements; work
+ * is enqueued on `stream` (a cudaStream_t) and the calls return without
+ * waiting and without allocating (the optimizer's first step uploads its
+ * table).  Outputs must not overlap inputs unless said.  Sums are held in
+ * float32; each stored value is rounded once.
+ *
+ * 8-bit matrices: e4m3 codes, 16-byte aligned with a pitch that is a multiple
+ * of 16 (the bytes between the width and the next multiple of 16 may be
+ * written), and one float32 scale for each block of 128 neighbouring entries
+ * of a row: scales[row][block], pitch at least ceil(width / 128).  A block z
+ * with A = max |z| holds the codes e4m3(448 z / A) (to nearest, ties to even)
+ * and the scale A / 448; a block with A < 2^-100 zero codes and scale 0.  A
+ * NaN makes its block NaN; an infinite A leaves zeros for finite entries and
+ * NaN for the infinite ones. */
+
+/* Root-mean-square norm with the residual's addition:
+ *   s = x + residual;  rstd = (mean(s^2) + eps)^-1/2;  y = s rstd weight.
+ * x, residual (may be NULL), sum (may be NULL; s, for the gradient and the
+ * next layer) and a wide y have type `dtype`; rstd (may be NULL) is
+ * float32[rows].  With `scales` non-NULL y goes to `out` in 8 bits, else as
+ * `dtype`.  In 8 bits rstd enters the scales alone (it is constant in a row
+ * and cancels from the codes), and the rule for tiny blocks looks at s weight. */
+int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride, const void* residual,
+                    int64_t residual_stride, int32_t dtype, const float* weight, double eps, void* sum,
+                    int64_t sum_stride, float* rstd, void* out, int64_t out_stride, float* scales,
+                    int64_t scale_stride, int32_t device, void* stream);
+
+/* Its gradient from s (`sum`) and rstd:
+ *   c = sum_d dy weight s;  dx = rstd weight dy - s rstd^3 c / width (+ dsum);
+ *   dweight = sum over rows of dy s rstd (float32, the same bits on every run).
+ * dsum (may be NULL) is the gradient that reaches s past the norm; dx is the
+ * gradient of x and of residual alike.  `workspace` holds at least
+ * mdsoap_rms_norm_backward_bytes bytes, 16-byte aligned. */
+int mdsoap_rms_norm_backward_bytes(int64_t rows, int64_t width, int32_t dtype, int32_t device, int64_t* bytes);
+int mdsoap_rms_norm_backward(const void* dy, int64_t rows, int64_t width, int64_t dy_stride, const void* sum,
+                             int64_t sum_stride, const float* rstd, const float* weight, const void* dsum,
+                             int64_t dsum_stride, int32_t dtype, void* dx, int64_t dx_stride, float* dweight,
+                             void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+
+/* 8-bit blocks of x[t][d] row_factor[t] col_factor[d] (factors may be NULL):
+ * along rows into codes [rows][code_stride] and scales [rows][ceil(width/128)],
+ * and / or along columns, transposed, into codes_t [width][code_t_stride] and
+ * scales_t [width][ceil(rows/128)]; either pair may be NULL.  A factor that is
+ * constant along a block enters its scale alone, sign and all.
+ * tiles != 0 (weights; no factors): one scale for each tile of 128 x 128,
+ * scales [ceil(rows/128)][ceil(width/128)] with the matrix as it is (may be
+ * NULL) and scales_t [ceil(width/128)][ceil(rows/128)] with its transpose. */
+int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride, int32_t dtype,
+                    const float* row_factor, const float* col_factor, int32_t tiles, void* codes, int64_t code_stride,
+                    float* scales, int64_t scale_stride, void* codes_t, int64_t code_t_stride, float* scales_t,
+                    int64_t scale_t_stride, int32_t device, void* stream);
+
+/* Product of two 8-bit matrices along their rows:
+ *   out[i][j] = sum_b a_scales[i][b] b_scales[j'][b] sum_{k in block b} a[i][k] b[j][k],
+ * j' = j / 128 with b_tiles (scales of 128 x 128 tiles), else j.  out is
+ * float32 or bfloat16 [m][out_stride]; accumulate != 0 adds to what out holds
+ * (float32 only).  `workspace` holds at least mdsoap_matmul_bytes bytes (which
+ * may be 0), 16-byte aligned. */
+int mdsoap_matmul_bytes(int64_t m, int64_t n, int64_t k, int32_t b_tiles, int32_t device, int64_t* bytes);
+int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_scales, int64_t a_scale_stride,
+                  const void* b, int64_t n, int64_t b_stride, const float* b_scales, int64_t b_scale_stride,
+                  int32_t b_tiles, int64_t k, int32_t out_dtype, int32_t accumulate, void* out, int64_t out_stride,
+                  void* workspace, int64_t workspace_bytes, int32_t device, void* stream);
+
+/* Wait for `stream` and report (and clear) a product on `device` whose copies
+ * or matrix instructions did not complete within their time limit. */
+int mdsoap_matmul_check(int32_t device, void* stream);
+
+/* AdamW over many tensors, one launch for every 448 of them:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2  (g times grad_scale);
+ *   p = p (1 - lr decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps).
+ * State of 32 bits: m and v float32.  State of 8 bits: e4m3 codes and one
+ * float32 scale for each 128 elements of a tensor, rounded by dithering with
+ * random numbers of (seed, step, element), the same on every run; a positive v
+ * keeps at least the smallest code.  Tensors are contiguous, of any alignment. */
+typedef struct mdsoap_adamw mdsoap_adamw;
+typedef struct {
+    int64_t tensors;
+    void* const* params;       /* of type dtype */
+    void* const* exp_avg;      /* m: float32, or e4m3 codes */
+    void* const* exp_avg_sq;   /* v: float32, or e4m3 codes */
+    float* const* exp_avg_scale;    /* 8 bits only: float32[ceil(count / 128)] */
+    float* const* exp_avg_sq_scale;
+    const int64_t* counts;
+    const float* weight_decay; /* one a tensor, or NULL for 0 */
+    int32_t dtype;             /* float32, bfloat16 or float16 */
+    int32_t state_bits;        /* 32 or 8 */
+    uint32_t seed;
+    int32_t device;
+} mdsoap_adamw_params;
+
+/* Checks and keeps the table of tensors; touches no GPU. */
+int mdsoap_adamw_create(const mdsoap_adamw_params* params, mdsoap_adamw** optimizer);
+/* One step (counted from 1) with the gradients, one a tensor, of grad_dtype. */
+int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t grad_dtype, int64_t step, double lr,
+                      double beta1, double beta2, double eps, double grad_scale, void* stream);
+void mdsoap_adamw_destroy(mdsoap_adamw* optimizer);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,8 @@ NOALLOC_SCRATCH_BYTES = 32 << 20  # MDSOAP_NOALLOC_SCRATCH_BYTES
 
 FLOAT32 = 0
 FLOAT64 = 1
+BFLOAT16 = 2
+FLOAT16 = 3
 AVERAGE = {"off": 0, "inner": 1, "outer": 2}
 COMPRESSION = {"off": 0, "mu2": 1, "mu1nu1": 2, "crossover": 3}
 WEIGHTING = {None: 0, "poly": 1, "pow": 2, "exp": 3}
@@ -77,6 +79,25 @@ class LocalParams(ctypes.Structure):
         ("species", ctypes.POINTER(ctypes.c_int32)),
         ("cutoff", ctypes.c_double),
         ("density_width", ctypes.c_double),
+    ]
+
+
+class AdamWParams(ctypes.Structure):
+    """``mdsoap_adamw_params`` (include/mdsoap.h)."""
+
+    _fields_ = [
+        ("tensors", ctypes.c_int64),
+        ("params", _P),
+        ("exp_avg", _P),
+        ("exp_avg_sq", _P),
+        ("exp_avg_scale", _P),
+        ("exp_avg_sq_scale", _P),
+        ("counts", _P),
+        ("weight_decay", _P),
+        ("dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("seed", ctypes.c_uint32),
+        ("device", ctypes.c_int32),
     ]
 
 
@@ -169,6 +190,20 @@ def _load() -> ctypes.CDLL:
     lib.mdsoap_local_feature_count.restype = ctypes.c_int64
     lib.mdsoap_local_compute.argtypes = [ctypes.POINTER(LocalParams), ctypes.POINTER(BatchView), _P, ctypes.c_int32]
     lib.mdsoap_local_compute.restype = ctypes.c_int
+    i32, i64, f64 = ctypes.c_int32, ctypes.c_int64, ctypes.c_double
+    lib.mdsoap_rms_norm.argtypes = [_P, i64, i64, i64, _P, i64, i32, _P, f64, _P, i64, _P, _P, i64, _P, i64, i32, _P]
+    lib.mdsoap_rms_norm_backward_bytes.argtypes = [i64, i64, i32, i32, ctypes.POINTER(i64)]
+    lib.mdsoap_rms_norm_backward.argtypes = [_P, i64, i64, i64, _P, i64, _P, _P, _P, i64, i32, _P, i64, _P, _P, i64,
+                                             i32, _P]
+    lib.mdsoap_quantize.argtypes = [_P, i64, i64, i64, i32, _P, _P, i32, _P, i64, _P, i64, _P, i64, _P, i64, i32, _P]
+    lib.mdsoap_matmul_bytes.argtypes = [i64, i64, i64, i32, i32, ctypes.POINTER(i64)]
+    lib.mdsoap_matmul.argtypes = [_P, i64, i64, _P, i64, _P, i64, i64, _P, i64, i32, i64, i32, i32, _P, i64, _P, i64,
+                                  i32, _P]
+    lib.mdsoap_matmul_check.argtypes = [i32, _P]
+    lib.mdsoap_adamw_create.argtypes = [ctypes.POINTER(AdamWParams), ctypes.POINTER(_P)]
+    lib.mdsoap_adamw_step.argtypes = [_P, _P, i32, i64, f64, f64, f64, f64, f64, _P]
+    lib.mdsoap_adamw_destroy.argtypes = [_P]
+    lib.mdsoap_adamw_destroy.restype = None
     return lib
 
 
@@ -212,6 +247,16 @@ EXPORTED = (
     "mdsoap_pairs_destroy",
     "mdsoap_local_feature_count",
     "mdsoap_local_compute",
+    "mdsoap_rms_norm",
+    "mdsoap_rms_norm_backward_bytes",
+    "mdsoap_rms_norm_backward",
+    "mdsoap_quantize",
+    "mdsoap_matmul_bytes",
+    "mdsoap_matmul",
+    "mdsoap_matmul_check",
+    "mdsoap_adamw_create",
+    "mdsoap_adamw_step",
+    "mdsoap_adamw_destroy",
 )
 
 

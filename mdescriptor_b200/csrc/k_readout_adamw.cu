@@ -1,0 +1,349 @@
+// AdamW over many tensors in one launch, with states in 32 bits or in 8, and
+// its C entry points (include/mdsoap.h).
+#include "readout_host.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <mutex>
+#include <vector>
+
+using namespace mdsoap;
+using namespace mdsoap::readout;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSpan = 4;                         // elements of one thread's unit
+constexpr int kTileUnits = 4;                    // units of a thread in one tile
+constexpr int kTile = kThreads * kSpan * kTileUnits;  // 4096 elements, a multiple of the block of 128
+constexpr int kGrads = 448;                      // gradient pointers handed over in one launch's parameters
+
+struct Tensor {
+    void* p;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t count;
+    int64_t first;  // position in the optimizer's own numbering of elements, a multiple of 128
+    float decay;    // weight decay
+    int32_t vector;  // p, m and v can be read in units of four
+};
+
+struct Tile {
+    int32_t tensor;
+    int32_t pad;
+    int64_t start;
+};
+
+struct StepArgs {
+    const Tensor* tensors;
+    const Tile* tiles;
+    int32_t first_tensor;  // of this launch: grads[0] belongs to it
+    float lr, beta1, beta2, rest1, rest2, eps, step_size, root2, grad_scale;
+    uint32_t key;
+    const void* grads[kGrads];
+};
+
+// Two 16-bit random numbers of an element: a counter mixed by two rounds of
+// shift, exclusive or and multiplication with odd constants (the fractional
+// parts of square roots of small primes).
+__device__ __forceinline__ uint32_t noise(int64_t element, uint32_t key) {
+    uint32_t h = (uint32_t)element ^ ((uint32_t)(element >> 32) * 0x3C6EF373u) ^ key;
+    h = (h ^ h >> 16) * 0xA54FF53Bu;
+    h = (h ^ h >> 15) * 0x510E527Fu;
+    return h ^ h >> 16;
+}
+
+// a >= 0 (at most 448) down to an e4m3 value after adding u / 2^16 of that
+// value's step.  Above 2^-6 the step is bit 20 of the float; below it is 2^-9.
+__device__ __forceinline__ float dither(float a, uint32_t u) {
+    const float normal = __uint_as_float((__float_as_uint(a) + (u << 4)) & 0xfff00000u);
+    const float low = floorf(fmaf((float)u, 0x1p-16f, a * 512.0f)) * 0x1p-9f;
+    return fminf(a >= 0x1p-6f ? normal : low, kTop);
+}
+
+template <class T>
+__device__ __forceinline__ void load4(const T* p, int64_t at, int64_t count, bool vector, float (&f)[4]) {
+    if (vector && at + 4 <= count) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(p + at);
+            f[0] = q.x, f[1] = q.y, f[2] = q.z, f[3] = q.w;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(p + at);
+            const T* t = reinterpret_cast<const T*>(&q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = to_float(t[i]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = at + i < count ? to_float(p[at + i]) : 0.0f;
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* p, int64_t at, int64_t count, bool vector, const float (&f)[4]) {
+    if (vector && at + 4 <= count) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(p + at) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+            uint2 q;
+            T* t = reinterpret_cast<T*>(&q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = from_float<T>(f[i]);
+            *reinterpret_cast<uint2*>(p + at) = q;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (at + i < count) p[at + i] = from_float<T>(f[i]);
+}
+
+__device__ __forceinline__ void load_codes4(const uint8_t* p, int64_t at, int64_t count, bool vector, float scale,
+                                            float (&f)[4]) {
+    uint32_t q = 0;
+    if (vector && at + 4 <= count) {
+        q = *reinterpret_cast<const uint32_t*>(p + at);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < count) q |= (uint32_t)p[at + i] << (8 * i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        __nv_fp8_e4m3 c;
+        c.__x = (uint8_t)(q >> (8 * i));
+        f[i] = (float)c * scale;
+    }
+}
+
+// New codes and scale of the warp's block of 128 values (four a lane).
+__device__ __forceinline__ void store_codes4(uint8_t* p, float* scales, int64_t at, int64_t count, bool vector,
+                                             const float (&x)[4], const uint32_t (&u)[4], bool positive) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(most, magnitude(x[i]));
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
+    const float scale = top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop);
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = __fdiv_rn(fabsf(x[i]), scale);
+        float c = dither(a, u[i]);
+        if (positive && c == 0.0f && x[i] > 0.0f) c = 0x1p-9f;
+        if (scale == 0.0f) c = 0.0f;
+        if (!(a == a) && scale != 0.0f) c = a;  // NaN stays
+        q[i] = copysignf(c, x[i]);
+    }
+    const uint32_t codes = codes4(q[0], q[1], q[2], q[3]);
+    if (vector && at + 4 <= count) {
+        *reinterpret_cast<uint32_t*>(p + at) = codes;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < count) p[at + i] = (uint8_t)(codes >> (8 * i));
+    }
+    if ((threadIdx.x & 31) == 0 && at < count) scales[at / kBlock] = scale;
+}
+
+// One CTA a tile of 4096 elements of one tensor.
+//   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// in float32, each stored value rounded once.
+// 8-bit states are e4m3 codes with a float32 scale for each block of 128
+// elements of the tensor; a warp holds exactly one block at a time.  They are
+// rounded by dithering: b2 = 0.999 moves v by a thousandth a step and the codes
+// lie 1/16 to 1/8 apart, so to the nearest code v would stay where it is.  v
+// itself is stored and not its root, whose dithering noise squared would add
+// to v more than b2 takes away; a positive v keeps at least the smallest code,
+// since a zero under a non-zero m would make a huge step.
+// Bound by HBM: p, m, v in and out, g in.
+template <class P, class G, bool SMALL>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const __grid_constant__ StepArgs a) {
+    const Tile tile = a.tiles[blockIdx.x];
+    const Tensor t = a.tensors[tile.tensor];
+    const G* g = static_cast<const G*>(a.grads[tile.tensor - a.first_tensor]);
+    P* p = static_cast<P*>(t.p);
+    const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
+    const float keep = 1.0f - a.lr * t.decay;
+#pragma unroll
+    for (int k = 0; k < kTileUnits; ++k) {
+        const int64_t at = tile.start + (k * kThreads + threadIdx.x) * kSpan;
+        if (tile.start + (k * kThreads + (threadIdx.x & ~31)) * kSpan >= t.count) break;  // the whole warp
+        float x[4], y[4], m[4], v[4];
+        load4(p, at, t.count, vec_p, x);
+        load4(g, at, t.count, vec_g, y);
+        if constexpr (SMALL) {
+            const int64_t block = min(at, t.count - 1) / kBlock;
+            load_codes4(static_cast<const uint8_t*>(t.m), at, t.count, vec_p, t.m_scale[block], m);
+            load_codes4(static_cast<const uint8_t*>(t.v), at, t.count, vec_p, t.v_scale[block], v);
+        } else {
+            load4(static_cast<const float*>(t.m), at, t.count, vec_p, m);
+            load4(static_cast<const float*>(t.v), at, t.count, vec_p, v);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float grad = y[i] * a.grad_scale;
+            // products rounded, then the sum: the states' codes depend on every bit of it
+            m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.rest1, grad));
+            v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(__fmul_rn(a.rest2, grad), grad));
+            x[i] = fmaf(-a.step_size, __fdiv_rn(m[i], fmaf(__fsqrt_rn(v[i]), a.root2, a.eps)), x[i] * keep);
+        }
+        store4(p, at, t.count, vec_p, x);
+        if constexpr (SMALL) {
+            uint32_t um[4], uv[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t h = noise(t.first + at + i, a.key);
+                um[i] = h >> 16, uv[i] = h & 0xffffu;
+            }
+            store_codes4(static_cast<uint8_t*>(t.m), t.m_scale, at, t.count, vec_p, m, um, false);
+            store_codes4(static_cast<uint8_t*>(t.v), t.v_scale, at, t.count, vec_p, v, uv, true);
+        } else {
+            store4(static_cast<float*>(t.m), at, t.count, vec_p, m);
+            store4(static_cast<float*>(t.v), at, t.count, vec_p, v);
+        }
+    }
+}
+
+}  // namespace
+
+struct mdsoap_adamw {
+    std::mutex mutex;
+    std::vector<Tensor> tensors;
+    std::vector<int64_t> tile_begin;  // [tensors + 1]
+    int32_t dtype = 0, state_bits = 32, device = 0;
+    uint32_t seed = 0;
+    void* table = nullptr;  // tensors, then tiles, on `device`
+    ~mdsoap_adamw() {
+        if (table) cudaFree(table);
+    }
+};
+
+namespace {
+
+// The table of tensors and tiles on the device, uploaded by the first step.
+void upload(mdsoap_adamw& o) {
+    if (o.table) return;
+    const int64_t tiles = o.tile_begin.back();
+    const size_t head = o.tensors.size() * sizeof(Tensor);
+    std::vector<unsigned char> host(head + tiles * sizeof(Tile));
+    std::copy_n(reinterpret_cast<const unsigned char*>(o.tensors.data()), head, host.data());
+    Tile* tile = reinterpret_cast<Tile*>(host.data() + head);
+    for (size_t i = 0; i < o.tensors.size(); ++i)
+        for (int64_t k = 0; k < o.tile_begin[i + 1] - o.tile_begin[i]; ++k) *tile++ = {(int32_t)i, 0, k * kTile};
+    void* table = nullptr;
+    check(engine_malloc(&table, host.size()), "optimizer table");
+    const cudaError_t err = cudaMemcpy(table, host.data(), host.size(), cudaMemcpyHostToDevice);
+    if (err != cudaSuccess) cudaFree(table);
+    check(err, "optimizer table upload");
+    o.table = table;
+}
+
+template <class P, class G>
+void launch(bool small, const StepArgs& a, unsigned tiles, cudaStream_t stream) {
+    if (small) adamw_kernel<P, G, true><<<tiles, kThreads, 0, stream>>>(a);
+    else adamw_kernel<P, G, false><<<tiles, kThreads, 0, stream>>>(a);
+    check(cudaGetLastError(), "optimizer launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mdsoap_adamw_create(const mdsoap_adamw_params* params, mdsoap_adamw** optimizer) {
+    if (!params || !optimizer) return fail(MDSOAP_INVALID_ARGUMENT, "null argument");
+    *optimizer = nullptr;
+    return entry([&] {
+        const mdsoap_adamw_params& q = *params;
+        need(q.tensors >= 0 && (q.tensors == 0 || (q.params && q.exp_avg && q.exp_avg_sq && q.counts)),
+             "readout: the optimizer needs its tensors");
+        need(q.state_bits == 32 || q.state_bits == 8, "readout: optimizer states take 32 or 8 bits");
+        need(q.state_bits == 32 || q.tensors == 0 || (q.exp_avg_scale && q.exp_avg_sq_scale),
+             "readout: 8-bit optimizer states need their scales");
+        by_type(q.dtype, [](auto) {});
+        auto o = std::make_unique<mdsoap_adamw>();
+        o->dtype = q.dtype;
+        o->state_bits = q.state_bits;
+        o->seed = q.seed;
+        o->device = q.device;
+        o->tile_begin.push_back(0);
+        int64_t first = 0;
+        const uintptr_t p_align = q.dtype == MDSOAP_FLOAT32 ? 16 : 8, state_align = q.state_bits == 32 ? 16 : 4;
+        for (int64_t i = 0; i < q.tensors; ++i) {
+            Tensor t{};
+            t.count = q.counts[i];
+            need(t.count >= 0, "readout: negative tensor size");
+            t.p = q.params[i];
+            t.m = q.exp_avg[i];
+            t.v = q.exp_avg_sq[i];
+            if (q.state_bits == 8) t.m_scale = q.exp_avg_scale[i], t.v_scale = q.exp_avg_sq_scale[i];
+            need(t.count == 0 || (t.p && t.m && t.v && (q.state_bits == 32 || (t.m_scale && t.v_scale))),
+                 "readout: null optimizer tensor");
+            t.first = first;
+            t.decay = q.weight_decay ? q.weight_decay[i] : 0.0f;
+            need(t.decay >= 0.0f, "readout: negative weight decay");
+            t.vector = (uintptr_t)t.p % p_align == 0 && (uintptr_t)t.m % state_align == 0 &&
+                       (uintptr_t)t.v % state_align == 0;
+            first += blocks_of(t.count) * kBlock;
+            o->tensors.push_back(t);
+            o->tile_begin.push_back(o->tile_begin.back() + (t.count + kTile - 1) / kTile);
+        }
+        need(o->tile_begin.back() <= 0x7fffffff, "readout: too many optimizer elements");
+        *optimizer = o.release();
+    });
+}
+
+void mdsoap_adamw_destroy(mdsoap_adamw* optimizer) { delete optimizer; }
+
+int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t grad_dtype, int64_t step, double lr,
+                      double beta1, double beta2, double eps, double grad_scale, void* stream) {
+    if (!optimizer) return fail(MDSOAP_INVALID_ARGUMENT, "null argument");
+    return entry([&] {
+        mdsoap_adamw& o = *optimizer;
+        need(step >= 1, "readout: optimizer steps count from 1");
+        need(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "readout: betas must lie in [0, 1)");
+        need(lr >= 0.0 && eps >= 0.0 && std::isfinite(lr) && std::isfinite(eps) && std::isfinite(grad_scale),
+             "readout: invalid optimizer settings");
+        need(grads || o.tensors.empty(), "readout: the optimizer step needs gradients");
+        for (size_t i = 0; i < o.tensors.size(); ++i)
+            need(grads[i] || o.tensors[i].count == 0, "readout: null gradient");
+        by_type(grad_dtype, [](auto) {});
+        if (o.tile_begin.back() == 0) return;
+        std::lock_guard<std::mutex> lock(o.mutex);
+        check(cudaSetDevice(o.device), "cudaSetDevice");
+        upload(o);
+        StepArgs a;
+        a.tensors = static_cast<const Tensor*>(o.table);
+        const Tile* tiles =
+            reinterpret_cast<const Tile*>(static_cast<const unsigned char*>(o.table) + o.tensors.size() * sizeof(Tensor));
+        a.lr = (float)lr;
+        a.beta1 = (float)beta1;
+        a.beta2 = (float)beta2;
+        a.rest1 = (float)(1.0 - beta1);
+        a.rest2 = (float)(1.0 - beta2);
+        a.eps = (float)eps;
+        a.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
+        a.root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+        a.grad_scale = (float)grad_scale;
+        a.key = o.seed * 0x6A09E667u + (uint32_t)step * 0xBB67AE85u;
+        for (size_t i = 0; i < o.tensors.size(); i += kGrads) {
+            const size_t end = std::min(o.tensors.size(), i + kGrads);
+            const int64_t count = o.tile_begin[end] - o.tile_begin[i];
+            if (count == 0) continue;
+            a.first_tensor = (int32_t)i;
+            a.tiles = tiles + o.tile_begin[i];
+            std::copy(grads + i, grads + end, a.grads);
+            by_type(o.dtype, [&](auto p) {
+                by_type(grad_dtype, [&](auto g) {
+                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)count,
+                                                     static_cast<cudaStream_t>(stream));
+                });
+            });
+        }
+    });
+}
+
+}  // extern "C"

@@ -5,6 +5,7 @@
 // there, so building a plan touches no GPU (the reference's construction-time
 // contract, tests/test_cuda_backend.py:266-279).
 #include "../../include/mdsoap.h"
+#include "host_errors.cuh"
 #include "launchers.cuh"
 #include "neighbor_list.cuh"
 #include "csr.cuh"
@@ -31,30 +32,6 @@ using namespace mdsoap;
 
 namespace {
 
-thread_local std::string g_error;
-
-int fail(int status, const std::string& message) {
-    g_error = message;
-    return status;
-}
-
-struct Failure {
-    int status;
-    std::string message;
-};
-
-[[noreturn]] void raise(int status, const std::string& message) { throw Failure{status, message}; }
-
-void check(cudaError_t err, const char* what) {
-    if (err == cudaSuccess) return;
-    const std::string text = std::string(what) + ": " + cudaGetErrorString(err);
-    if (err == cudaErrorMemoryAllocation) raise(MDSOAP_OUT_OF_MEMORY, text);
-    if (err == cudaErrorNoDevice || err == cudaErrorInsufficientDriver || err == cudaErrorInvalidDevice ||
-        err == cudaErrorDevicesUnavailable || err == cudaErrorInitializationError)
-        raise(MDSOAP_DEVICE_UNAVAILABLE, text);
-    raise(MDSOAP_INTERNAL, text);
-}
-
 std::string device_error_text(unsigned bits) {
     if (bits & kErrUnknownSpecies) return "batch contains an atomic number outside calculator species";
     if (bits & kErrMixedPbc) return "mixed periodicity is not supported; use all-zero or all-one pbc";
@@ -65,22 +42,6 @@ std::string device_error_text(unsigned bits) {
     if (bits & kErrTailTimeout) return "tail kernel: a coefficient block copy did not complete in time";
     if (bits & kErrLocalSeries) return "local descriptor radial integral overflow";
     return "device error";
-}
-
-// Injected allocation failure, for the out-of-memory tests: with
-// MDSOAP_TEST_FAIL_ALLOC=<bytes> set, every engine device allocation of at
-// least that many bytes returns cudaErrorMemoryAllocation without calling
-// cudaMalloc, so the OUT_OF_MEMORY path (status, plugin exception, adapter
-// error code) is exercised on the host, with no real exhaustion of a GPU.
-cudaError_t engine_malloc(void** ptr, size_t bytes) {
-    if (const char* env = std::getenv("MDSOAP_TEST_FAIL_ALLOC")) {
-        const long long limit = std::atoll(env);
-        if (limit > 0 && bytes >= (size_t)limit) {
-            *ptr = nullptr;
-            return cudaErrorMemoryAllocation;
-        }
-    }
-    return cudaMalloc(ptr, bytes);
 }
 
 // Host-side NVTX range (upload, binning, expansion, tail, D2H), closed at scope exit.

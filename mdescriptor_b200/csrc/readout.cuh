@@ -1,0 +1,216 @@
+// Device-side pieces shared by the readout operators: 16-byte units of a row
+// at any alignment, e4m3 blocks of 128, element types.
+//
+// A block of 128 entries z with A = max |z| is stored as the codes
+// e4m3(448 z / A) and the float32 scale A / 448; a block with A < 2^-100 as
+// zero codes with scale 0.  A NaN in a block makes A and so the whole block
+// NaN; an infinite A leaves zeros for the finite entries and NaN for the rest.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace mdsoap {
+namespace readout {
+
+constexpr int kBlock = 128;
+constexpr float kTop = 448.0f;      // largest e4m3 value
+constexpr float kTiny = 0x1p-100f;  // blocks below it are zeros: 448 / A stays far inside float32
+
+inline int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+// ------------------------------------------------------------ element types
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// ------------------------------------------------------------ 16-byte units
+
+// Elements of T in one 16-byte unit.
+template <class T>
+constexpr int kUnit = 16 / (int)sizeof(T);
+
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[kUnit<T>]) {
+    const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) f[i] = to_float(t[i]);
+}
+
+template <class T>
+__device__ __forceinline__ uint4 pack(const float (&f)[kUnit<T>]) {
+    uint4 u;
+    T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) t[i] = from_float<T>(f[i]);
+    return u;
+}
+
+// Bytes [shift, shift + 16) of the 32 bytes a, b; 0 < shift < 16, the same in
+// all lanes of a warp.
+__device__ __forceinline__ uint4 splice(const uint4& a, const uint4& b, int shift) {
+    uint32_t w0, w1, w2, w3, w4;
+    switch (shift >> 2) {
+        case 0: w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x; break;
+        case 1: w0 = a.y, w1 = a.z, w2 = a.w, w3 = b.x, w4 = b.y; break;
+        case 2: w0 = a.z, w1 = a.w, w2 = b.x, w3 = b.y, w4 = b.z; break;
+        default: w0 = a.w, w1 = b.x, w2 = b.y, w3 = b.z, w4 = b.w; break;
+    }
+    const int r = (shift & 3) * 8;
+    return make_uint4(__funnelshift_r(w0, w1, r), __funnelshift_r(w1, w2, r), __funnelshift_r(w2, w3, r),
+                      __funnelshift_r(w3, w4, r));
+}
+
+// A read-only matrix with unit column stride.  [begin, end) is the byte range
+// its elements span: the two aligned words that hold a misaligned unit are
+// only read where both lie inside it.
+template <class T>
+struct MatrixIn {
+    const T* data;
+    int64_t rows, width, stride;
+
+    __device__ __forceinline__ uint4 unit(int64_t row, int64_t col) const {
+        if (col >= width) return make_uint4(0, 0, 0, 0);
+        const T* p = data + row * stride + col;
+        if (col + kUnit<T> <= width) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+            const int shift = (int)(at & 15);
+            if (shift == 0) return __ldg(reinterpret_cast<const uint4*>(p));
+            const uintptr_t begin = reinterpret_cast<uintptr_t>(data);
+            const uintptr_t end = reinterpret_cast<uintptr_t>(data + (rows - 1) * stride + width);
+            const uintptr_t word = at - shift;
+            if (word >= begin && word + 32 <= end) {
+                const uint4* w = reinterpret_cast<const uint4*>(word);
+                return splice(__ldg(w), __ldg(w + 1), shift);
+            }
+        }
+        uint4 u = make_uint4(0, 0, 0, 0);
+        T* t = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int i = 0; i < kUnit<T>; ++i)
+            if (col + i < width) t[i] = p[i];
+        return u;
+    }
+};
+
+// A row store of one unit per lane; the lanes of a warp hold consecutive units
+// (lane l the elements col .. col + kUnit).  All 32 lanes call it together.
+// Where the row is not 16-byte aligned, each lane joins its unit's head to its
+// lower neighbour's tail and stores that aligned word; the two ends of the
+// warp's stretch go out element by element.
+template <class T>
+__device__ __forceinline__ void store_unit(T* row, int64_t col, int64_t width, const uint4& u) {
+    T* p = row + col;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);  // uniform: col is a multiple of the unit
+    const T* t = reinterpret_cast<const T*>(&u);
+    const bool full = col + kUnit<T> <= width;
+    if (shift == 0) {
+        if (full) {
+            *reinterpret_cast<uint4*>(p) = u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kUnit<T>; ++i)
+                if (col + i < width) p[i] = t[i];
+        }
+        return;
+    }
+    uint4 below;
+    below.x = __shfl_up_sync(0xffffffffu, u.x, 1);
+    below.y = __shfl_up_sync(0xffffffffu, u.y, 1);
+    below.z = __shfl_up_sync(0xffffffffu, u.z, 1);
+    below.w = __shfl_up_sync(0xffffffffu, u.w, 1);
+    const int lane = threadIdx.x & 31;
+    const int head = (16 - shift) / (int)sizeof(T);  // elements of a unit below the next aligned word
+    if (lane > 0 && col + head <= width) {
+        // the aligned word ends `head` elements into this lane's unit
+        *reinterpret_cast<uint4*>(p + head - kUnit<T>) = splice(below, u, 16 - shift);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kUnit<T>; ++i) {
+            // head of this unit, and (when the word was cut off) the neighbour's tail
+            if (i < head && col + i < width) p[i] = t[i];
+        }
+        if (lane > 0) {
+            const T* b = reinterpret_cast<const T*>(&below);
+#pragma unroll
+            for (int i = 0; i < kUnit<T>; ++i)
+                if (i >= head && col - kUnit<T> + i < width) p[i - kUnit<T>] = b[i];
+        }
+    }
+    if (lane == 31) {
+#pragma unroll
+        for (int i = 0; i < kUnit<T>; ++i)
+            if (i >= head && col + i < width) p[i] = t[i];
+    }
+}
+
+// kUnit<T> float32 values of a vector from `col` on; zero past `width`.
+template <int N>
+__device__ __forceinline__ void load_vector(const float* v, int64_t col, int64_t width, float (&f)[N]) {
+    const float* p = v + col;
+    if (col + N <= width && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(p + i));
+            f[i] = q.x, f[i + 1] = q.y, f[i + 2] = q.z, f[i + 3] = q.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = col + i < width ? __ldg(p + i) : 0.0f;
+}
+
+// ------------------------------------------------------------ blocks of 128
+
+// |x| as an unsigned whose order is the magnitudes' with NaN on top.
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// 448 / top as a sum hi + lo, so that fma(z, hi, z * lo) is the correctly
+// rounded quotient's neighbour to within 2^-40: an entry that lies on a tie
+// between two codes is seen as one.  Zero for a block that is stored as zeros.
+struct Factor {
+    float hi, lo;
+    __device__ __forceinline__ explicit Factor(float top) {
+        if (top < kTiny) {
+            hi = lo = 0.0f;
+            return;
+        }
+        hi = __fdiv_rn(kTop, top);
+        lo = top == INFINITY ? 0.0f : __fdiv_rn(fmaf(-hi, top, kTop), top);
+    }
+    __device__ __forceinline__ float operator()(float z) const { return fmaf(z, hi, z * lo); }
+};
+
+__device__ __forceinline__ float scale_of(float top) { return top < kTiny ? 0.0f : __fdiv_rn(top, kTop); }
+
+// Two e4m3 codes, `a` in the low byte.
+__device__ __forceinline__ uint32_t codes2(float a, float b) {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+    return codes2(a, b) | codes2(c, d) << 16;
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+
+}  // namespace readout
+}  // namespace mdsoap

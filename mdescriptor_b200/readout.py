@@ -1,0 +1,374 @@
+"""Operators of a readout: a network trained on SOAP rows and asked for answers.
+
+Rows of ``Soap.compute_device`` go through a residual stream that is normalised
+and stored in 8 bits (``rms_norm``), 8-bit matrix products whose scales belong
+to blocks of 128 (``quantize``, ``matmul``), their gradients
+(``rms_norm_backward``, and ``matmul`` on blocks along columns) and an AdamW
+step over all tensors at once (``AdamW``).  The kernels are those of
+libmdsoap.so; torch tensors hold the memory.  Every call runs on the current
+stream of its tensors' device and returns without waiting.
+
+One layer y = rms_norm(x + r) W^T and its gradients::
+
+    weight = quantize(w, layout="tiles")                  # .rows is W, .columns its transpose
+    n = rms_norm(x, g, residual=r, output="float8")       # n.output (blocks), n.sum, n.rstd
+    y = matmul(n.output, weight.rows)
+    d = quantize(dy, layout="both")
+    x8 = quantize(n.sum, layout="columns", row_factor=n.rstd, col_factor=g)   # normalised rows, transposed
+    dw = matmul(d.columns, x8.columns, dtype="float32")
+    dn = matmul(d.rows, weight.columns)
+    dx, dg = rms_norm_backward(dn, n.sum, n.rstd, g, dsum=dsum)
+"""
+
+from __future__ import annotations
+
+import ctypes
+from functools import lru_cache
+from typing import NamedTuple, Sequence
+
+import torch
+
+from . import _lib
+from ._lib import AdamWParams, lib, raise_for
+
+BLOCK = 128
+
+_DTYPES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
+_NAMES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+_CODES = torch.float8_e4m3fn
+
+
+class Blocks(NamedTuple):
+    """An 8-bit matrix: e4m3 ``values`` [rows, width] (row pitch a multiple of
+    16) and float32 ``scales`` [rows, ceil(width / 128)], or
+    [ceil(rows / 128), ceil(width / 128)] where they belong to tiles."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def float(self) -> torch.Tensor:
+        """The float32 values that the codes stand for."""
+        rows, width = self.values.shape
+        scales = self.scales.repeat_interleave(BLOCK, dim=1)[:, :width]
+        if scales.shape[0] != rows:
+            scales = scales.repeat_interleave(BLOCK, dim=0)[:rows]
+        return self.values.float() * scales
+
+
+class Quantized(NamedTuple):
+    """Result of ``quantize``: ``rows`` is the matrix, ``columns`` its
+    transpose, each in blocks along its own rows (None where not asked for)."""
+
+    rows: Blocks | None
+    columns: Blocks | None
+
+
+class Norm(NamedTuple):
+    """Result of ``rms_norm``: ``output`` (``Blocks`` or a tensor), the sum
+    x + residual (x itself without a residual) and the row factors ``rstd``."""
+
+    output: "Blocks | torch.Tensor"
+    sum: torch.Tensor
+    rstd: torch.Tensor
+
+
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _matrix(x: torch.Tensor, name: str) -> tuple[int, int, int]:
+    """(rows, width, row pitch) of a 2-D CUDA tensor with unit column stride."""
+    if x.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    rows, width = x.shape
+    stride, unit = x.stride()
+    if unit != 1 and width > 1:
+        raise ValueError(f"{name} must have unit column stride, got strides {x.stride()}")
+    if rows > 1 and stride < width:
+        raise ValueError(f"{name} has rows that overlap (strides {x.stride()})")
+    return rows, width, max(stride, width)
+
+
+def _dtype(x: torch.Tensor, name: str) -> int:
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {x.dtype}")
+    return code
+
+
+def _vector(x: torch.Tensor | None, count: int, like: torch.Tensor, name: str) -> int | None:
+    if x is None:
+        return None
+    if x.dtype != torch.float32 or x.shape != (count,) or not x.is_contiguous() or x.device != like.device:
+        raise ValueError(f"{name} must be a contiguous float32 vector of {count} on {like.device}")
+    return x.data_ptr()
+
+
+def _same(x: torch.Tensor, like: torch.Tensor, name: str) -> int:
+    """Row pitch of a matrix with the shape, type and device of ``like``."""
+    if x.shape != like.shape or x.dtype != like.dtype or x.device != like.device:
+        raise ValueError(f"{name} must have shape {tuple(like.shape)}, type {like.dtype} and device {like.device}")
+    return _matrix(x, name)[2]
+
+
+def _empty_blocks(rows: int, width: int, scale_rows: int, device: torch.device) -> Blocks:
+    blocks = (width + BLOCK - 1) // BLOCK
+    pitch, scale_pitch = (width + 15) // 16 * 16, (blocks + 3) // 4 * 4
+    values = torch.empty((rows, pitch), dtype=_CODES, device=device)
+    scales = torch.empty((scale_rows, scale_pitch), dtype=torch.float32, device=device)
+    return Blocks(values if pitch == width else values[:, :width],
+                  scales if scale_pitch == blocks else scales[:, :blocks])
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+             output: str | None = None) -> Norm:
+    """y = s (mean(s^2) + eps)^-1/2 weight of each row, s = x + residual.
+
+    ``output`` "float8": y in 8 bits (``Blocks``); None: y in x's type.  ``sum``
+    is s in x's type (x itself without a residual); with ``rstd`` it is what
+    ``rms_norm_backward`` takes."""
+    if output not in (None, "float8"):
+        raise ValueError("output must be None or 'float8'")
+    rows, width, stride = _matrix(x, "x")
+    dtype = _dtype(x, "x")
+    weight_ptr = _vector(weight, width, x, "weight")
+    residual_stride = 0 if residual is None else _same(residual, x, "residual")
+    total = x if residual is None else torch.empty((rows, width), dtype=x.dtype, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    if output is None:
+        out: Blocks | torch.Tensor = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        out_ptr, out_stride, scales_ptr, scale_stride = out.data_ptr(), width, None, 0
+    else:
+        out = _empty_blocks(rows, width, rows, x.device)
+        out_ptr, out_stride = out.values.data_ptr(), out.values.stride(0)
+        scales_ptr, scale_stride = out.scales.data_ptr(), out.scales.stride(0)
+        if rows == 0 or width == 0:
+            scales_ptr = scales_ptr or 16  # no element is touched; the form stays 8-bit
+    raise_for(lib.mdsoap_rms_norm(
+        x.data_ptr(), rows, width, stride, None if residual is None else residual.data_ptr(), residual_stride, dtype,
+        weight_ptr, eps, None if residual is None else total.data_ptr(), width, rstd.data_ptr(), out_ptr, out_stride,
+        scales_ptr, scale_stride, x.device.index, _stream(x.device.index)))
+    return Norm(out, total, rstd)
+
+
+@lru_cache(maxsize=1024)
+def _norm_backward_bytes(rows: int, width: int, dtype: int, device: int) -> int:
+    value = ctypes.c_int64()
+    raise_for(lib.mdsoap_rms_norm_backward_bytes(rows, width, dtype, device, ctypes.byref(value)))
+    return value.value
+
+
+def rms_norm_backward(dy: torch.Tensor, sum: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor,
+                      dsum: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) of ``rms_norm`` from its ``sum`` and ``rstd``.
+
+    ``dsum`` is the gradient that reaches the sum past the norm (the residual
+    stream's); dx is the gradient of x and of residual alike.  An 8-bit output
+    passes its gradient through unchanged.  dweight is float32 and the same bits
+    on every run."""
+    rows, width, stride = _matrix(sum, "sum")
+    dtype = _dtype(sum, "sum")
+    dy_stride = _same(dy, sum, "dy")
+    dsum_stride = 0 if dsum is None else _same(dsum, sum, "dsum")
+    rstd_ptr = _vector(rstd, rows, sum, "rstd")
+    weight_ptr = _vector(weight, width, sum, "weight")
+    device = sum.device.index
+    bytes_ = _norm_backward_bytes(rows, width, dtype, device)
+    dx = torch.empty((rows, width), dtype=sum.dtype, device=sum.device)
+    dweight = torch.empty(width, dtype=torch.float32, device=sum.device)
+    workspace = torch.empty(bytes_, dtype=torch.uint8, device=sum.device)
+    raise_for(lib.mdsoap_rms_norm_backward(
+        dy.data_ptr(), rows, width, dy_stride, sum.data_ptr(), stride, rstd_ptr, weight_ptr,
+        None if dsum is None else dsum.data_ptr(), dsum_stride, dtype, dx.data_ptr(), width, dweight.data_ptr(),
+        workspace.data_ptr(), bytes_, device, _stream(device)))
+    return dx, dweight
+
+
+def quantize(x: torch.Tensor, layout: str = "rows", row_factor: torch.Tensor | None = None,
+             col_factor: torch.Tensor | None = None) -> Quantized:
+    """8-bit blocks of x * row_factor[:, None] * col_factor.
+
+    ``layout`` "rows": blocks along rows; "columns": of the transpose; "both":
+    both from one read of x; "tiles" (weights): one scale for each tile of
+    128 x 128, the matrix and its transpose."""
+    if layout not in ("rows", "columns", "both", "tiles"):
+        raise ValueError("layout must be 'rows', 'columns', 'both' or 'tiles'")
+    rows, width, stride = _matrix(x, "x")
+    dtype = _dtype(x, "x")
+    row_ptr = _vector(row_factor, rows, x, "row_factor")
+    col_ptr = _vector(col_factor, width, x, "col_factor")
+    tiles = layout == "tiles"
+    if tiles and (row_ptr or col_ptr):
+        raise ValueError("tiles take no factors")
+    by_rows = by_columns = None
+    args: list = [None, 0, None, 0, None, 0, None, 0]
+    if layout != "columns":
+        by_rows = _empty_blocks(rows, width, (rows + BLOCK - 1) // BLOCK if tiles else rows, x.device)
+        args[:4] = (by_rows.values.data_ptr(), by_rows.values.stride(0), by_rows.scales.data_ptr(),
+                    by_rows.scales.stride(0))
+    if layout != "rows":
+        by_columns = _empty_blocks(width, rows, (width + BLOCK - 1) // BLOCK if tiles else width, x.device)
+        args[4:] = (by_columns.values.data_ptr(), by_columns.values.stride(0), by_columns.scales.data_ptr(),
+                    by_columns.scales.stride(0))
+    if rows and width:
+        raise_for(lib.mdsoap_quantize(x.data_ptr(), rows, width, stride, dtype, row_ptr, col_ptr, int(tiles), *args,
+                                      x.device.index, _stream(x.device.index)))
+    return Quantized(by_rows, by_columns)
+
+
+def _blocks(b: Blocks, name: str, tiles: bool) -> tuple[int, int, int, int, bool]:
+    """(rows, width, pitch, scale pitch, scales of tiles) of checked blocks."""
+    values, scales = b
+    rows, width, stride = _matrix(values, f"{name}.values")
+    if values.dtype != _CODES:
+        raise ValueError(f"{name}.values must be float8_e4m3fn, got {values.dtype}")
+    scale_rows, blocks, scale_stride = _matrix(scales, f"{name}.scales")
+    if scales.dtype != torch.float32 or scales.device != values.device:
+        raise ValueError(f"{name}.scales must be float32 on {values.device}")
+    by_rows = scale_rows == rows
+    if blocks != (width + BLOCK - 1) // BLOCK or not (by_rows or (tiles and scale_rows == (rows + BLOCK - 1) // BLOCK)):
+        raise ValueError(f"{name}.scales has shape {tuple(scales.shape)}, which fits no blocks of {tuple(values.shape)}")
+    if rows and width and (stride % 16 or values.data_ptr() % 16):
+        raise ValueError(f"{name}.values must start on 16 bytes and have a row pitch that is a multiple of 16")
+    return rows, width, stride, scale_stride, not by_rows
+
+
+@lru_cache(maxsize=4096)
+def _matmul_bytes(m: int, n: int, k: int, tiles: bool, device: int) -> int:
+    value = ctypes.c_int64()
+    raise_for(lib.mdsoap_matmul_bytes(m, n, k, int(tiles), device, ctypes.byref(value)))
+    return value.value
+
+
+def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | None = None,
+           accumulate: bool = False) -> torch.Tensor:
+    """a b^T [m, n] of two 8-bit matrices with blocks along their common width.
+
+    ``b`` may carry scales of tiles (weights) or of its rows (the weight's
+    gradient).  ``dtype`` "bfloat16" or "float32"; ``out`` takes the result, and
+    with ``accumulate`` (float32) has it added."""
+    m, k, a_stride, a_scale_stride, _ = _blocks(a, "a", False)
+    n, k_b, b_stride, b_scale_stride, tiles = _blocks(b, "b", True)
+    if k != k_b:
+        raise ValueError(f"a and b must have the same width, got {k} and {k_b}")
+    device = a.values.device
+    if b.values.device != device:
+        raise ValueError("a and b must be on the same device")
+    if out is None:
+        if dtype not in ("bfloat16", "float32"):
+            raise ValueError("dtype must be 'bfloat16' or 'float32'")
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty((m, n), dtype=_NAMES[dtype], device=device)
+        out_stride = n
+    else:
+        if out.shape != (m, n) or out.device != device or out.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"out must be a bfloat16 or float32 matrix of shape {(m, n)} on {device}")
+        out_stride = _matrix(out, "out")[2]
+        if accumulate and out.dtype != torch.float32:
+            raise ValueError("accumulate needs a float32 out")
+    bytes_ = _matmul_bytes(m, n, k, tiles, device.index)
+    workspace = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
+    raise_for(lib.mdsoap_matmul(
+        a.values.data_ptr(), m, a_stride, a.scales.data_ptr(), a_scale_stride, b.values.data_ptr(), n, b_stride,
+        b.scales.data_ptr(), b_scale_stride, int(tiles), k, _DTYPES[out.dtype], int(accumulate), out.data_ptr(),
+        out_stride, None if workspace is None else workspace.data_ptr(), bytes_, device.index, _stream(device.index)))
+    return out
+
+
+def check(device: int = 0) -> None:
+    """Wait for the current stream and raise if a product on ``device`` gave up waiting."""
+    raise_for(lib.mdsoap_matmul_check(int(device), _stream(device)))
+
+
+class AdamW:
+    """AdamW over all of a readout's tensors in one launch.
+
+    ``params``: contiguous CUDA tensors of one type (float32, bfloat16 or
+    float16), updated in place.  ``state_bits`` 32 holds both moments in
+    float32; 8 holds them as e4m3 codes with a scale for each 128 elements,
+    rounded by dithering with random numbers of (seed, step, element).
+    ``weight_decay``: one number, or one a tensor.  ``state``: moments to
+    continue from (``exp_avg``, ``exp_avg_sq``, with 8 bits ``exp_avg_scale``
+    and ``exp_avg_sq_scale``: lists like ``params``; ``step``: the steps
+    taken), used in place; ``self.state`` has the same form."""
+
+    def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float | Sequence[float] = 0.01, state_bits: int = 32, seed: int = 0,
+                 state: dict | None = None) -> None:
+        self._optimizer = None
+        self.params = list(params)
+        self.lr, self.betas, self.eps = float(lr), (float(betas[0]), float(betas[1])), float(eps)
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self.state_bits = state_bits
+        if not self.params:
+            raise ValueError("AdamW needs at least one tensor")
+        first = self.params[0]
+        for p in self.params:
+            if not p.is_cuda or not p.is_contiguous() or p.dtype != first.dtype or p.device != first.device:
+                raise ValueError("params must be contiguous CUDA tensors of one type on one device")
+        dtype = _dtype(first, "params")
+        self.device = first.device
+        self._counts = [p.numel() for p in self.params]
+        count = len(self.params)
+        decays = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        if len(decays) != count:
+            raise ValueError("weight_decay must be one number or one a tensor")
+        kind = _CODES if state_bits == 8 else torch.float32
+        blocks = [(n + BLOCK - 1) // BLOCK for n in self._counts]
+        if state is None:
+            state = {"step": 0}
+            for key in ("exp_avg", "exp_avg_sq"):
+                state[key] = [torch.zeros(n, dtype=torch.uint8, device=self.device).view(_CODES) if state_bits == 8 else
+                              torch.zeros(n, dtype=kind, device=self.device) for n in self._counts]
+                if state_bits == 8:
+                    state[key + "_scale"] = [torch.zeros(n, dtype=torch.float32, device=self.device) for n in blocks]
+        self.state = {"step": int(state["step"])}
+        arrays = {"params": self.params}
+        for key in ("exp_avg", "exp_avg_sq"):
+            for name, sizes, want in ((key, self._counts, kind),
+                                      (key + "_scale", blocks, torch.float32))[:2 if state_bits == 8 else 1]:
+                tensors = list(state[name])
+                if len(tensors) != count or any(t.numel() != n or t.dtype != want or t.device != self.device or
+                                                not t.is_contiguous() for t, n in zip(tensors, sizes)):
+                    raise ValueError(f"state {name!r} must hold {count} contiguous {want} tensors that fit the params")
+                self.state[name] = arrays[name] = tensors
+        pointers = {key: (ctypes.c_void_p * count)(*[t.data_ptr() for t in v]) for key, v in arrays.items()}
+        counts = (ctypes.c_int64 * count)(*self._counts)
+        decay = (ctypes.c_float * count)(*decays)
+        address = {key: ctypes.cast(v, ctypes.c_void_p) for key, v in pointers.items()}
+        handle = ctypes.c_void_p()
+        raise_for(lib.mdsoap_adamw_create(ctypes.byref(AdamWParams(
+            count, address["params"], address["exp_avg"], address["exp_avg_sq"], address.get("exp_avg_scale"),
+            address.get("exp_avg_sq_scale"), ctypes.cast(counts, ctypes.c_void_p), ctypes.cast(decay, ctypes.c_void_p),
+            dtype, state_bits, int(seed) & 0xFFFFFFFF, self.device.index)), ctypes.byref(handle)))
+        self._optimizer = handle
+
+    def step(self, grads: Sequence[torch.Tensor], lr: float | None = None, grad_scale: float = 1.0) -> None:
+        """Update every tensor with its gradient (one type for all, times ``grad_scale``)."""
+        grads = list(grads)
+        if [g.numel() for g in grads] != self._counts:
+            raise ValueError("grads must be one tensor for each of params, of its size")
+        dtype = grads[0].dtype
+        if any(g.dtype != dtype or not g.is_contiguous() or g.device != self.device for g in grads):
+            raise ValueError(f"grads must be contiguous tensors of one type on {self.device}")
+        step = self.state["step"] + 1
+        raise_for(lib.mdsoap_adamw_step(
+            self._optimizer, (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads]), _dtype(grads[0], "grads"),
+            step, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, grad_scale,
+            _stream(self.device.index)))
+        self.state["step"] = step
+
+    def close(self) -> None:
+        if self._optimizer:
+            lib.mdsoap_adamw_destroy(self._optimizer)
+            self._optimizer = None
+
+    def __del__(self) -> None:
+        try:
+            self.close()
+        except Exception:
+            pass
