@@ -1,5 +1,12 @@
 // Product of two 8-bit matrices with scales for blocks of 128 on the tensor
 // cores, and its C entry points (include/mdsoap.h).
+//
+//   out[i][j] = sum_b sa[i][b] sb[j'][b] (sum over k in block b of a[i][k] b[j][k])
+//
+// The inner sums are matrix instructions over 128 bytes of K into tensor memory.
+// Their scales change from block to block, so each block's partial product is
+// taken out of tensor memory, multiplied and added in float32 registers, while
+// the next block fills the other accumulator.
 #include "readout_host.cuh"
 #include "tcgen05.cuh"
 
@@ -10,11 +17,8 @@ using namespace mdsoap::readout;
 
 namespace {
 
-constexpr int kTileM = 128;
 constexpr int kTileK = 128;  // bytes of K a stage: one scale block
-constexpr int kStages = 6;
-constexpr int kPromote = 8;                       // warps that scale and add the partial products
-constexpr int kThreads = (kPromote + 2) * 32;     // and one each for the copies and the matrix instructions
+constexpr int kRows = 128;   // rows of one CTA's accumulator: the lanes of tensor memory
 
 __device__ unsigned g_gave_up;  // products whose copies or matrix instructions did not complete in time
 
@@ -24,21 +28,29 @@ struct ProductArgs {
     int64_t a_scale_stride;
     const float* b_scales;
     int64_t b_scale_stride;
+    int32_t b_tiles;
     void* out;
     int64_t out_stride;
     int32_t accumulate;
+    int32_t splits;   // parts of K, each a work item of its own
+    float* partials;  // [split][tile][256][256] where splits > 1
 };
 
-template <int BN>
-struct Shared {
-    uint8_t a[kStages][kTileM * kTileK];
-    uint8_t b[kStages][BN * kTileK];
-    float b_scale[2][BN];
-    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
-    uint32_t tensor_memory;
-    int gave_up;
-    int issued;
-};
+// Four neighbouring scales of a row from block `b` on; zero from block `end` on.
+__device__ __forceinline__ float4 scales4(const float* row, int b, int end, bool vector) {
+    if (vector && b + 4 <= end) return __ldg(reinterpret_cast<const float4*>(row + b));
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (b < end) f.x = row[b];
+    if (b + 1 < end) f.y = row[b + 1];
+    if (b + 2 < end) f.z = row[b + 2];
+    if (b + 3 < end) f.w = row[b + 3];
+    return f;
+}
+
+__device__ __forceinline__ float pick(const float4& f, int i) {
+    const float low = i & 1 ? f.y : f.x, high = i & 1 ? f.w : f.z;
+    return i & 2 ? high : low;
+}
 
 // COUNT neighbouring results of one row; `left` of them lie inside the matrix.
 template <class OUT, int COUNT>
@@ -69,21 +81,55 @@ __device__ __forceinline__ void store_row(OUT* p, int64_t left, const float (&f)
     }
 }
 
-// One CTA a tile of 128 x BN.  One thread copies tiles of A and B (one block of
-// 128 of K a stage) into swizzled shared memory, one issues the matrix
-// instructions of a block into one of two accumulators in tensor memory, and
-// eight warps take each block's partial product out, multiply it by its scales
-// and add it in float32 registers, while the other accumulator fills.
-template <int BN, bool TILES, class OUT>
-__global__ __launch_bounds__(kThreads, 1) void product_kernel(const __grid_constant__ CUtensorMap map_a,
-                                                              const __grid_constant__ CUtensorMap map_b,
-                                                              const __grid_constant__ ProductArgs p) {
-    extern __shared__ __align__(1024) uint8_t raw[];
-    Shared<BN>& s = *reinterpret_cast<Shared<BN>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    constexpr int kColumns = 2 * BN;
+// ------------------------------------------------------------ pairs of CTAs
+//
+// A pair of CTAs (two SMs) computes a tile of 256 x 256: each holds 128 rows of
+// A and of B in shared memory and 128 rows of the accumulators, and the pair's
+// matrix instructions read both halves of B, so each SM copies and reads only
+// half of it.  A single SM's 128 x 256 tile would move 48 KB through shared
+// memory for every 128 of K where this moves 32 KB; at the tensor cores' rate
+// that is what shared memory can deliver.
+// Per CTA: warp 8 copies tiles of A and B (one block of K a stage), warp 9 of
+// the first CTA issues the matrix instructions, warps 0 to 7 scale and add.
+// Persistent: the pairs take tiles (and parts of K) in turn, columns first, so
+// that the pairs at work share A's rows and B stays in L2.
+
+constexpr int kPairTile = 256;
+constexpr int kPromote = 8;                    // warps that scale and add the partial products
+constexpr int kThreads = (kPromote + 4) * 32;  // a warp each for the copies and the matrix instructions, two to fill up
+// Registers: launched with 168 a thread; the last four warps give theirs up to 72
+// and the other eight take 216 (8 x 216 + 4 x 72 = 12 x 168).
+constexpr int kManyRegisters = 216, kFewRegisters = 72;
+
+enum class Store { Tile, Direct, Partial };
+
+template <bool TILES>
+struct PairShared {
+    static constexpr int kStages = TILES ? 6 : 5;
+    uint8_t a[kStages][kRows * kTileK];
+    uint8_t b[kStages][kRows * kTileK];
+    uint8_t out[kPromote][32 * 128];  // one 128-byte piece of each of a warp's rows on its way out
+    float b_scale[TILES ? 1 : 2][4][TILES ? 4 : kPairTile];
+    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
+    uint32_t tensor_memory;
+    int gave_up;
+    int issued;
+};
+
+template <bool TILES, class OUT, Store STORE>
+__global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                                   const __grid_constant__ CUtensorMap map_b,
+                                                                   const __grid_constant__ CUtensorMap map_out,
+                                                                   const __grid_constant__ ProductArgs p) {
+    extern __shared__ uint8_t raw[];
+    using S = PairShared<TILES>;
+    constexpr int kStages = S::kStages;
+    S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t m0 = (int64_t)blockIdx.y * kTileM, n0 = (int64_t)blockIdx.x * BN;
+    const int rank = (int)tc::cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
     const int blocks = (int)((p.k + kTileK - 1) / kTileK);
+    const int tiles_n = (int)((p.n + kPairTile - 1) / kPairTile), tiles_m = (int)((p.m + kPairTile - 1) / kPairTile);
+    const int tiles = tiles_n * tiles_m, items = tiles * p.splits;  // the host keeps them below 2^30
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
@@ -92,115 +138,402 @@ __global__ __launch_bounds__(kThreads, 1) void product_kernel(const __grid_const
         }
         for (int i = 0; i < 2; ++i) {
             bulk::barrier_init(&s.acc_full[i], 1);
-            bulk::barrier_init(&s.acc_empty[i], kPromote);
+            bulk::barrier_init(&s.acc_empty[i], 2 * kPromote);
         }
         bulk::barrier_init(&s.drained, 1);
         s.gave_up = 0;
         s.issued = 0;
         bulk::barrier_init_fence();
     }
-    if (warp == kPromote + 1) tc::alloc(&s.tensor_memory, kColumns);
+    if (warp == kPromote + 1) tc::alloc<2>(&s.tensor_memory, 512);
     tc::fence_before();
     __syncthreads();
+    tc::cluster_sync();
     tc::fence_after();
     const uint32_t tmem = *(volatile uint32_t*)&s.tensor_memory;
     volatile int* gave_up = &s.gave_up;
 
-    if (warp == kPromote) {
-        if (lane == 0) {
-            int kb = 0;
-            for (; kb < blocks; ++kb) {
-                const int stage = kb % kStages;
-                if (!tc::wait(&s.empty[stage], (kb / kStages & 1) ^ 1, gave_up)) break;
-                bulk::arrive_expect(&s.full[stage], (kTileM + BN) * kTileK);
-                tc::load_tile(s.a[stage], &map_a, kb * kTileK, (int)m0, &s.full[stage]);
-                tc::load_tile(s.b[stage], &map_b, kb * kTileK, (int)n0, &s.full[stage]);
+    // The tile and the part of K of a work item.
+    const auto item_m = [&](int item) { return item % tiles / tiles_n * kPairTile; };
+    const auto item_n = [&](int item) { return item % tiles % tiles_n * kPairTile; };
+    const auto first_block = [&](int item) { return (int)((int64_t)(item / tiles) * blocks / p.splits); };
+    const auto last_block = [&](int item) { return (int)((int64_t)(item / tiles + 1) * blocks / p.splits); };
+
+    if (warp >= kPromote) {
+        tc::give_registers<kFewRegisters>();
+        if (warp == kPromote && lane == 0) {
+            int count = 0;
+            bool good = true;
+            for (int item = pair; item < items && good; item += pairs) {
+                const int m0 = item_m(item) + rank * kRows, n0 = item_n(item) + rank * kRows;
+                const int end = last_block(item);
+                for (int kb = first_block(item); kb < end; ++kb, ++count) {
+                    const int stage = count % kStages;
+                    if (!tc::wait(&s.empty[stage], (count / kStages & 1) ^ 1, gave_up)) {
+                        good = false;
+                        break;
+                    }
+                    const uint32_t full = tc::map_shared(&s.full[stage], 0);
+                    if (rank == 0) bulk::arrive_expect(&s.full[stage], 4 * kRows * kTileK);
+                    tc::load_tile_pair(s.a[stage], &map_a, kb * kTileK, m0, full);
+                    tc::load_tile_pair(s.b[stage], &map_b, kb * kTileK, n0, full);
+                }
             }
-            s.issued = kb;
-        }
-    } else if (warp == kPromote + 1) {
-        if (lane == 0) {
-            constexpr uint32_t word = tc::instruction(kTileM, BN);
-            for (int kb = 0; kb < blocks; ++kb) {
-                const int stage = kb % kStages, buffer = kb & 1;
-                if (!tc::wait(&s.acc_empty[buffer], (kb >> 1 & 1) ^ 1, gave_up)) break;
-                if (!tc::wait(&s.full[stage], kb / kStages & 1, gave_up)) break;
-                tc::fence_after();
-                const uint64_t a = tc::operand(s.a[stage]), b = tc::operand(s.b[stage]);
+            s.issued = count;
+        } else if (warp == kPromote + 1 && lane == 0 && rank == 0) {
+            constexpr uint32_t word = tc::instruction(kPairTile, kPairTile);
+            int count = 0;
+            for (int item = pair; item < items && !*gave_up; item += pairs) {
+                const int end = last_block(item);
+                for (int kb = first_block(item); kb < end; ++kb, ++count) {
+                    const int stage = count % kStages, buffer = count & 1;
+                    if (!tc::wait(&s.acc_empty[buffer], (count >> 1 & 1) ^ 1, gave_up)) break;
+                    if (!tc::wait(&s.full[stage], count / kStages & 1, gave_up)) break;
+                    tc::fence_after();
+                    const uint64_t a = tc::operand(s.a[stage]), b = tc::operand(s.b[stage]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc::mma(tmem + buffer * BN, a + 2 * k, b + 2 * k, word, k > 0);
-                tc::commit(&s.empty[stage]);
-                tc::commit(&s.acc_full[buffer]);
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma<2>(tmem + buffer * kPairTile, a + 2 * k, b + 2 * k, word, k > 0);
+                    tc::commit<2>(&s.empty[stage]);
+                    tc::commit<2>(&s.acc_full[buffer]);
+                }
             }
             if (*gave_up) {  // matrix instructions in flight end before the tensor memory goes
-                tc::commit(&s.drained);
+                tc::commit<2>(&s.drained);
                 bulk::wait(&s.drained, 0);
             }
         }
     } else {
-        constexpr int kMine = BN / 2;  // columns of one thread
+        tc::take_registers<kManyRegisters>();
+        constexpr int kMine = kPairTile / 2;  // columns of one thread
         const int quarter = warp & 3, half = warp >> 2;
-        const int64_t row = m0 + quarter * 32 + lane;
-        const int64_t col = n0 + half * kMine;
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * kMine;
-        float acc[kMine];
+        const bool vec_a = p.a_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.a_scales) % 16 == 0;
+        const bool vec_b = p.b_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.b_scales) % 16 == 0;
+        int count = 0;
+        for (int item = pair; item < items; item += pairs) {
+            const int m0 = item_m(item) + rank * kRows, n0 = item_n(item);
+            const int begin = first_block(item), end = last_block(item);
+            const int row = m0 + quarter * 32 + lane, col = n0 + half * kMine;
+            // a row or column past the matrix takes scales of one that exists; its results are never stored
+            const float* sa = p.a_scales + min(row, (int)p.m - 1) * p.a_scale_stride;
+            const float* sb = p.b_scales +
+                              (TILES ? min(col, (int)p.n - 1) / kBlock : min(n0 + (int)threadIdx.x, (int)p.n - 1)) *
+                                  p.b_scale_stride;
+            uint64_t acc[kMine / 2];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) acc[i] = 0.0f;
-        const bool live = row < p.m;
-        const float* sa = p.a_scales + (live ? row : 0) * p.a_scale_stride;
-        const int64_t b_row = TILES ? min(col, p.n - 1) / kBlock : n0 + threadIdx.x;
-        const bool b_live = TILES || (threadIdx.x < BN && b_row < p.n);
-        const float* sb = p.b_scales + (b_live ? b_row : 0) * p.b_scale_stride;
-        float next_a = live && blocks ? sa[0] : 0.0f, next_b = b_live && blocks ? sb[0] : 0.0f;
-        for (int kb = 0; kb < blocks; ++kb) {
-            const int buffer = kb & 1;
-            const float scale_a = next_a, scale_b = next_b;
-            if (kb + 1 < blocks) {
-                if (live) next_a = sa[kb + 1];
-                if (b_live) next_b = sb[kb + 1];
-            }
-            if constexpr (!TILES) {
-                if (threadIdx.x < BN) s.b_scale[buffer][threadIdx.x] = scale_b;
-                asm volatile("bar.sync 1, %0;" ::"n"(kPromote * 32) : "memory");
-            }
-            if (!tc::wait(&s.acc_full[buffer], kb >> 1 & 1, gave_up)) *gave_up = 1;
-            __syncwarp();
-            tc::fence_after();
-#pragma unroll
-            for (int c = 0; c < kMine; c += 32) {
-                uint32_t part[32];
-                tc::load32(from + buffer * BN + c, part);
-                tc::wait_loads();
-                if (c + 32 == kMine) {
-                    tc::fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::arrive(&s.acc_empty[buffer]);
+            for (int i = 0; i < kMine / 2; ++i) acc[i] = 0;  // two zeros
+            float4 next_a = scales4(sa, begin & ~3, end, vec_a), next_b = scales4(sb, begin & ~3, end, vec_b);
+            float4 scale = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int kb = begin; kb < end; ++kb, ++count) {
+                const int buffer = count & 1, group = kb >> 2 & 1;
+                if (kb == begin || (kb & 3) == 0) {  // the scales of four blocks at a time, loaded four blocks ahead
+                    if constexpr (TILES) {
+                        scale = make_float4(next_a.x * next_b.x, next_a.y * next_b.y, next_a.z * next_b.z,
+                                            next_a.w * next_b.w);
+                    } else {
+                        scale = next_a;
+                        s.b_scale[group][0][threadIdx.x] = next_b.x;
+                        s.b_scale[group][1][threadIdx.x] = next_b.y;
+                        s.b_scale[group][2][threadIdx.x] = next_b.z;
+                        s.b_scale[group][3][threadIdx.x] = next_b.w;
+                        asm volatile("bar.sync 1, %0;" ::"n"(kPromote * 32) : "memory");
+                    }
+                    next_a = scales4(sa, (kb & ~3) + 4, end, vec_a);
+                    next_b = scales4(sb, (kb & ~3) + 4, end, vec_b);
                 }
-                if constexpr (TILES) {
-                    const float scale = scale_a * scale_b;
+                const float mine = pick(scale, kb & 3);
+                const uint64_t mine2 = tc::pair_of(mine, mine);
+                tc::wait(&s.acc_full[buffer], count >> 1 & 1, gave_up);
+                __syncwarp();
+                tc::fence_after();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[c + i] = fmaf(__uint_as_float(part[i]), scale, acc[c + i]);
-                } else {
+                for (int c = 0; c < kMine; c += 32) {
+                    uint32_t part[32];
+                    tc::load32(from + buffer * kPairTile + c, part);
+                    tc::wait_loads();
+                    if (c + 32 == kMine) {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::arrive_at(tc::map_shared(&s.acc_empty[buffer], 0));
+                    }
+                    if constexpr (TILES) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        acc[c + i] = fmaf(__uint_as_float(part[i]), scale_a * s.b_scale[buffer][half * kMine + c + i],
-                                          acc[c + i]);
+                        for (int i = 0; i < 16; ++i)
+                            acc[c / 2 + i] = tc::fma2(
+                                tc::pair_of(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])), mine2,
+                                acc[c / 2 + i]);
+                    } else {
+                        const ulonglong2* sb2 =
+                            reinterpret_cast<const ulonglong2*>(&s.b_scale[group][kb & 3][half * kMine + c]);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const ulonglong2 q = sb2[i / 2];
+                            acc[c / 2 + i] = tc::fma2(
+                                tc::pair_of(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])),
+                                tc::mul2(mine2, q.x), acc[c / 2 + i]);
+                            acc[c / 2 + i + 1] = tc::fma2(
+                                tc::pair_of(__uint_as_float(part[2 * i + 2]), __uint_as_float(part[2 * i + 3])),
+                                tc::mul2(mine2, q.y), acc[c / 2 + i + 1]);
+                        }
+                    }
+                }
+            }
+            if (*gave_up) break;
+            if constexpr (STORE == Store::Partial) {
+                float* out = p.partials + ((int64_t)item * kPairTile + rank * kRows + quarter * 32 + lane) * kPairTile + half * kMine;
+#pragma unroll
+                for (int i = 0; i < kMine / 2; i += 2)
+                    *reinterpret_cast<ulonglong2*>(out + 2 * i) = make_ulonglong2(acc[i], acc[i + 1]);
+            } else if constexpr (STORE == Store::Tile) {
+                // 128 bytes of each of the warp's rows at a time: 16-byte pieces in the swizzled order the
+                // copy engine expects (piece ^ row % 8), so that neither side meets bank conflicts
+                constexpr int kWide = 128 / (int)sizeof(OUT);
+                uint8_t* mine_out = s.out[warp] + lane * 128;
+#pragma unroll
+                for (int c = 0; c < kMine; c += kWide) {
+                    if (lane == 0) tc::wait_store_reads();
+                    __syncwarp();
+#pragma unroll
+                    for (int piece = 0; piece < 8; ++piece) {
+                        constexpr int kEach = 16 / (int)sizeof(OUT);
+                        float f[kEach];
+#pragma unroll
+                        for (int i = 0; i < kEach; i += 2)
+                            tc::split_pair(acc[(c + piece * kEach + i) / 2], f[i], f[i + 1]);
+                        uint4 q;
+                        OUT* t = reinterpret_cast<OUT*>(&q);
+#pragma unroll
+                        for (int i = 0; i < kEach; ++i) t[i] = from_float<OUT>(f[i]);
+                        *reinterpret_cast<uint4*>(mine_out + ((piece ^ (lane & 7)) * 16)) = q;
+                    }
+                    bulk::proxy_fence();
+                    __syncwarp();
+                    if (lane == 0 && m0 + quarter * 32 < p.m && col + c < p.n)
+                        tc::store_tile(&map_out, col + c, m0 + quarter * 32, s.out[warp]);
+                }
+            } else {
+                if (row < p.m) {
+                    OUT* out = static_cast<OUT*>(p.out) + (int64_t)row * p.out_stride + col;
+#pragma unroll
+                    for (int c = 0; c < kMine; c += 32) {
+                        float f[32];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) tc::split_pair(acc[c / 2 + i], f[2 * i], f[2 * i + 1]);
+                        store_row(out + c, p.n - col - c, f, p.accumulate);
+                    }
                 }
             }
         }
-        if (live && !*gave_up)
-            store_row(static_cast<OUT*>(p.out) + row * p.out_stride + col, p.n - col, acc, p.accumulate);
+        if (STORE == Store::Tile && lane == 0) tc::wait_stores();
     }
 
     __syncthreads();
     if (*gave_up && threadIdx.x == 0) {
         atomicOr(&g_gave_up, 1u);
         // copies in flight land before the shared memory goes
-        for (int kb = max(0, s.issued - kStages); kb < s.issued; ++kb)
-            bulk::wait(&s.full[kb % kStages], kb / kStages & 1);
+        if (rank == 0)
+            for (int i = max(0, s.issued - kStages); i < s.issued; ++i)
+                bulk::wait(&s.full[i % kStages], i / kStages & 1);
     }
+    tc::cluster_sync();  // neither CTA leaves while the other may still reach into its memory
+    if (warp == kPromote + 1) tc::dealloc<2>(tmem, 512);
+}
+
+// out = the parts' partial products in order.
+template <class OUT>
+__global__ __launch_bounds__(256) void add_parts_kernel(const __grid_constant__ ProductArgs p) {
+    const int tiles_n = (int)((p.n + kPairTile - 1) / kPairTile), tiles_m = (int)((p.m + kPairTile - 1) / kPairTile);
+    const int64_t part = (int64_t)tiles_n * tiles_m * kPairTile * kPairTile;
+    const int64_t col = (blockIdx.x * 64ll + threadIdx.x % 64) * 4, row = blockIdx.y * 4ll + threadIdx.x / 64;
+    if (row >= p.m || col >= p.n) return;
+    const float* from = p.partials + ((row / kPairTile * tiles_n + col / kPairTile) * kPairTile + row % kPairTile) * kPairTile +
+                        col % kPairTile;
+    float4 sum = *reinterpret_cast<const float4*>(from);
+#pragma unroll 4
+    for (int i = 1; i < p.splits; ++i) {
+        const float4 q = *reinterpret_cast<const float4*>(from + i * part);
+        sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+    }
+    const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+    store_row(static_cast<OUT*>(p.out) + row * p.out_stride + col, p.n - col, f, p.accumulate);
+}
+
+// ------------------------------------------------------------ few rows
+//
+// With at most 128 rows of A the product reads B once and is bound by that.
+// Here B's rows are the lanes: a CTA takes 128 of them and all rows of A (padded
+// to COLS) as the columns, so each 16 KB of B travel beside COLS / 8 KB of A.
+// The CTAs of a cluster share K, each adds up its part, and they join their sums
+// through each other's shared memory in the cluster's order.
+
+constexpr int kFewThreads = 6 * 32;  // four warps that scale and add, one for the copies, one for the instructions
+
+template <int COLS>
+struct FewShared {  // at most 224 KB
+    static constexpr int kStages = COLS <= 32 ? 8 : COLS == 64 ? 7 : 4;
+    uint8_t b[kStages][kRows * kTileK];
+    uint8_t a[kStages][COLS * kTileK];
+    float a_scale[2][4][COLS];
+    float sum[COLS][kRows];
+    uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
+    uint32_t tensor_memory;
+    int gave_up;
+    int issued;
+};
+
+template <int COLS, class OUT>
+__global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                                     const __grid_constant__ CUtensorMap map_b,
+                                                                     const __grid_constant__ ProductArgs p) {
+    extern __shared__ uint8_t raw[];
+    using S = FewShared<COLS>;
+    constexpr int kStages = S::kStages;
+    constexpr int kColumns = 2 * COLS < 32 ? 32 : 2 * COLS;
+    S& s = *reinterpret_cast<S*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)tc::cluster_rank(), parts = p.splits;
+    const int blocks = (int)((p.k + kTileK - 1) / kTileK);
+    const int n0 = (int)(blockIdx.x / parts) * kRows;
+    const int begin = (int)((int64_t)rank * blocks / parts), end = (int)((int64_t)(rank + 1) * blocks / parts);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            bulk::barrier_init(&s.full[i], 1);
+            bulk::barrier_init(&s.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bulk::barrier_init(&s.acc_full[i], 1);
+            bulk::barrier_init(&s.acc_empty[i], 4);
+        }
+        bulk::barrier_init(&s.drained, 1);
+        s.gave_up = 0;
+        s.issued = 0;
+        bulk::barrier_init_fence();
+    }
+    if (warp == 5) tc::alloc<1>(&s.tensor_memory, kColumns);
+    tc::fence_before();
     __syncthreads();
-    if (warp == kPromote + 1) tc::dealloc(tmem, kColumns);
+    tc::fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)&s.tensor_memory;
+    volatile int* gave_up = &s.gave_up;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            int count = 0;
+            for (int kb = begin; kb < end; ++kb, ++count) {
+                const int stage = count % kStages;
+                if (!tc::wait(&s.empty[stage], (count / kStages & 1) ^ 1, gave_up)) break;
+                bulk::arrive_expect(&s.full[stage], (kRows + COLS) * kTileK);
+                tc::load_tile(s.b[stage], &map_b, kb * kTileK, n0, &s.full[stage]);
+                tc::load_tile(s.a[stage], &map_a, kb * kTileK, 0, &s.full[stage]);
+            }
+            s.issued = count;
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            constexpr uint32_t word = tc::instruction(kRows, COLS);
+            int count = 0;
+            for (int kb = begin; kb < end; ++kb, ++count) {
+                const int stage = count % kStages, buffer = count & 1;
+                if (!tc::wait(&s.acc_empty[buffer], (count >> 1 & 1) ^ 1, gave_up)) break;
+                if (!tc::wait(&s.full[stage], count / kStages & 1, gave_up)) break;
+                tc::fence_after();
+                const uint64_t b = tc::operand(s.b[stage]), a = tc::operand(s.a[stage]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc::mma<1>(tmem + buffer * COLS, b + 2 * k, a + 2 * k, word, k > 0);
+                tc::commit<1>(&s.empty[stage]);
+                tc::commit<1>(&s.acc_full[buffer]);
+            }
+            if (*gave_up) {
+                tc::commit<1>(&s.drained);
+                bulk::wait(&s.drained, 0);
+            }
+        }
+    } else {
+        const int64_t n = n0 + threadIdx.x;
+        const float* sb = p.b_scales + min(n, p.n - 1) / (p.b_tiles ? kBlock : 1) * p.b_scale_stride;
+        const bool vec_a = p.a_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.a_scales) % 16 == 0;
+        const bool vec_b = p.b_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.b_scales) % 16 == 0;
+        const bool loader = threadIdx.x < COLS;
+        const float* sa = p.a_scales + min((int64_t)threadIdx.x, p.m - 1) * p.a_scale_stride;
+        uint64_t acc[COLS / 2];
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) acc[i] = 0;
+        float4 next_b = scales4(sb, begin & ~3, end, vec_b), scale = next_b;
+        float4 next_a = loader ? scales4(sa, begin & ~3, end, vec_a) : scale;
+        int count = 0;
+        for (int kb = begin; kb < end; ++kb, ++count) {
+            const int buffer = count & 1, group = kb >> 2 & 1;
+            if (kb == begin || (kb & 3) == 0) {
+                scale = next_b;
+                if (loader) {
+                    s.a_scale[group][0][threadIdx.x] = next_a.x;
+                    s.a_scale[group][1][threadIdx.x] = next_a.y;
+                    s.a_scale[group][2][threadIdx.x] = next_a.z;
+                    s.a_scale[group][3][threadIdx.x] = next_a.w;
+                    next_a = scales4(sa, (kb & ~3) + 4, end, vec_a);
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                next_b = scales4(sb, (kb & ~3) + 4, end, vec_b);
+            }
+            const float mine = pick(scale, kb & 3);
+            const uint64_t mine2 = tc::pair_of(mine, mine);
+            tc::wait(&s.acc_full[buffer], count >> 1 & 1, gave_up);
+            __syncwarp();
+            tc::fence_after();
+            const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + buffer * COLS;
+            constexpr int kStep = COLS < 32 ? COLS : 32;
+#pragma unroll
+            for (int c = 0; c < COLS; c += kStep) {
+                uint32_t part[kStep];
+                tc::load(from + c, part);
+                tc::wait_loads();
+                if (c + kStep == COLS) {
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc::arrive(&s.acc_empty[buffer]);
+                }
+                const ulonglong2* sa2 = reinterpret_cast<const ulonglong2*>(&s.a_scale[group][kb & 3][c]);
+#pragma unroll
+                for (int i = 0; i < kStep / 2; i += 2) {
+                    const ulonglong2 q = sa2[i / 2];
+                    acc[c / 2 + i] =
+                        tc::fma2(tc::pair_of(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])),
+                                 tc::mul2(mine2, q.x), acc[c / 2 + i]);
+                    acc[c / 2 + i + 1] =
+                        tc::fma2(tc::pair_of(__uint_as_float(part[2 * i + 2]), __uint_as_float(part[2 * i + 3])),
+                                 tc::mul2(mine2, q.y), acc[c / 2 + i + 1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < COLS / 2; ++i) {
+            float x, y;
+            tc::split_pair(acc[i], x, y);
+            s.sum[2 * i][threadIdx.x] = x;
+            s.sum[2 * i + 1][threadIdx.x] = y;
+        }
+    }
+
+    __syncthreads();
+    if (*gave_up && threadIdx.x == 0) {
+        atomicOr(&g_gave_up, 1u);
+        for (int i = max(0, s.issued - kStages); i < s.issued; ++i) bulk::wait(&s.full[i % kStages], i / kStages & 1);
+    }
+    tc::cluster_sync();
+    const int64_t n = n0 + threadIdx.x;
+    if (threadIdx.x < kRows && n < p.n && !*gave_up) {
+        for (int64_t j = rank; j < p.m; j += parts) {
+            float sum = 0.0f;
+#pragma unroll 8
+            for (int r = 0; r < parts; ++r) sum += tc::load_shared_at(tc::map_shared(&s.sum[j][threadIdx.x], r));
+            OUT* out = static_cast<OUT*>(p.out) + j * p.out_stride + n;
+            *out = from_float<OUT>(p.accumulate ? to_float(*out) + sum : sum);
+        }
+    }
+    tc::cluster_sync();  // the others may still read this CTA's sums
+    if (warp == 5) tc::dealloc<1>(tmem, kColumns);
 }
 
 // ------------------------------------------------------------ host
@@ -223,26 +556,124 @@ EncodeTiled encoder() {
     return f;
 }
 
-CUtensorMap tile_map(const void* base, int64_t rows, int64_t k, int64_t stride, int box_rows) {
+// Pieces of 128 bytes x `box_rows` rows of a matrix, swizzled in shared memory.
+CUtensorMap tile_map(CUtensorMapDataType type, int size, const void* base, int64_t rows, int64_t cols, int64_t stride,
+                     int box_rows) {
     CUtensorMap map;
-    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)std::max<int64_t>(stride, 16)};
-    const cuuint32_t box[2] = {kTileK, (cuuint32_t)box_rows}, steps[2] = {1, 1};
-    if (encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)std::max<int64_t>(stride * size, 16)};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    if (encoder()(&map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         raise(MDSOAP_INVALID_ARGUMENT, "readout: a product's operand cannot be described to the copy engine");
     return map;
 }
+CUtensorMap code_map(const void* base, int64_t rows, int64_t k, int64_t stride, int box_rows) {
+    return tile_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k, stride, box_rows);
+}
 
-template <int BN, bool TILES, class OUT>
-void launch_product(const CUtensorMap& a, const CUtensorMap& b, const ProductArgs& p, cudaStream_t stream) {
-    auto kernel = product_kernel<BN, TILES, OUT>;
-    constexpr int bytes = sizeof(Shared<BN>) + 1024;
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "product shared memory");
-    const dim3 grid((unsigned)((p.n + BN - 1) / BN), (unsigned)((p.m + kTileM - 1) / kTileM));
-    kernel<<<grid, kThreads, bytes, stream>>>(a, b, p);
-    check(cudaGetLastError(), "product launch");
+template <class K, class... Args>
+void launch(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t bytes, cudaStream_t stream,
+            const Args&... args) {
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "product shared memory");
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = cluster;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = bytes;
+    config.stream = stream;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    check(cudaLaunchKernelEx(&config, kernel, args...), "product launch");
+}
+
+// What a product of this shape runs.
+struct Shape {
+    bool few;
+    int columns;  // few rows: A's rows, padded
+    int splits;
+    int64_t tiles;
+    int64_t bytes;
+};
+
+Shape shape_of(int64_t m, int64_t n, int64_t k, int sms) {
+    Shape s{};
+    const int64_t blocks = blocks_of(k);
+    s.few = m <= kRows;
+    s.splits = 1;
+    if (s.few) {
+        s.columns = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+        s.tiles = blocks_of(n);
+        // up to eight CTAs (the portable cluster) share K while SMs are free and each keeps two blocks
+        while (s.splits < 8 && s.tiles * s.splits * 2 <= sms && blocks >= s.splits * 4) s.splits *= 2;
+        return s;
+    }
+    s.tiles = ((m + kPairTile - 1) / kPairTile) * ((n + kPairTile - 1) / kPairTile);
+    // Parts of K where whole tiles leave pairs idle.  In units of one block's time: rounds of the busiest pair, each
+    // with 6 blocks' time around its sum, and for more than one part a second kernel that takes about 10 blocks'
+    // time and reads every part of every tile, 1/60 of a block's time each.
+    need(s.tiles < (1 << 25), "readout: product too large");
+    const int64_t pairs = sms / 2;
+    double best = 0.0;
+    for (int64_t parts = 1; parts <= 32 && (parts == 1 || blocks >= parts * 4); ++parts) {
+        const double rounds = (double)((s.tiles * parts + pairs - 1) / pairs);
+        const double time = rounds * ((double)((blocks + parts - 1) / parts) + 6.0) +
+                            (parts > 1 ? 10.0 + (double)(s.tiles * parts) / 60.0 : 0.0);
+        if (parts == 1 || time < best) best = time, s.splits = (int)parts;
+    }
+    if (s.splits > 1) s.bytes = s.tiles * s.splits * kPairTile * kPairTile * (int64_t)sizeof(float);
+    return s;
+}
+
+template <int COLS, class OUT>
+void run_few(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
+             cudaStream_t stream) {
+    const CUtensorMap map_a = code_map(a, p.m, p.k, a_stride, COLS), map_b = code_map(b, p.n, p.k, b_stride, kRows);
+    launch(few_product_kernel<COLS, OUT>, (unsigned)(s.tiles * s.splits), (unsigned)s.splits, kFewThreads,
+           sizeof(FewShared<COLS>) + 1024, stream, map_a, map_b, p);
+}
+
+template <bool TILES, class OUT>
+void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
+               int sms, cudaStream_t stream) {
+    const CUtensorMap map_a = code_map(a, p.m, p.k, a_stride, kRows), map_b = code_map(b, p.n, p.k, b_stride, kRows);
+    const unsigned grid = 2 * (unsigned)std::min<int64_t>(sms / 2, s.tiles * s.splits);
+    const size_t bytes = sizeof(PairShared<TILES>) + 1024;
+    if (s.splits > 1) {
+        launch(pair_product_kernel<TILES, float, Store::Partial>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_a, p);
+        const dim3 add((unsigned)((p.n + 255) / 256), (unsigned)((p.m + 3) / 4));
+        add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
+        check(cudaGetLastError(), "product launch");
+    } else if (!p.accumulate && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 &&
+               (p.out_stride * sizeof(OUT)) % 16 == 0) {
+        const CUtensorMap map_out =
+            tile_map(sizeof(OUT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(OUT),
+                     p.out, p.m, p.n, p.out_stride, 32);
+        launch(pair_product_kernel<TILES, OUT, Store::Tile>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_out, p);
+    } else {
+        launch(pair_product_kernel<TILES, OUT, Store::Direct>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_a, p);
+    }
+}
+
+template <class OUT>
+void run_product(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
+                 int sms, cudaStream_t stream) {
+    if (s.few) {
+        switch (s.columns) {
+            case 16: run_few<16, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
+            case 32: run_few<32, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
+            case 64: run_few<64, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
+            default: run_few<128, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
+        }
+    } else if (p.b_tiles) {
+        run_pairs<true, OUT>(a, a_stride, b, b_stride, p, s, sms, stream);
+    } else {
+        run_pairs<false, OUT>(a, a_stride, b, b_stride, p, s, sms, stream);
+    }
 }
 
 }  // namespace
@@ -252,9 +683,8 @@ extern "C" {
 int mdsoap_matmul_bytes(int64_t m, int64_t n, int64_t k, int32_t b_tiles, int32_t device, int64_t* bytes) {
     return entry([&] {
         need(m >= 0 && n >= 0 && k >= 0 && bytes, "readout: invalid product shape");
-        (void)b_tiles;
-        (void)device;
-        *bytes = 0;
+        (void)b_tiles;  // the same work for both forms
+        *bytes = m == 0 || n == 0 || k == 0 ? 0 : shape_of(m, n, k, sm_count(device)).bytes;
     });
 }
 
@@ -285,19 +715,16 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
             if (!accumulate) check(cudaMemset2DAsync(out, std::max(out_stride, n) * size, 0, n * size, m, s), "clear");
             return;
         }
-        (void)workspace;
-        (void)workspace_bytes;
-        constexpr int BN = 128;
-        need((m + kTileM - 1) / kTileM <= 65535, "readout: too many rows in a product");
-        const CUtensorMap map_a = tile_map(a, m, k, a_stride, kTileM), map_b = tile_map(b, n, k, b_stride, BN);
-        const ProductArgs p{m, n, k, a_scales, a_scale_stride, b_scales, b_scale_stride, out, out_stride, accumulate};
-        if (out_dtype == MDSOAP_FLOAT32) {
-            if (b_tiles) launch_product<BN, true, float>(map_a, map_b, p, s);
-            else launch_product<BN, false, float>(map_a, map_b, p, s);
-        } else {
-            if (b_tiles) launch_product<BN, true, __nv_bfloat16>(map_a, map_b, p, s);
-            else launch_product<BN, false, __nv_bfloat16>(map_a, map_b, p, s);
-        }
+        const int sms = sm_count(device);
+        const Shape shape = shape_of(m, n, k, sms);
+        need(shape.bytes == 0 || (workspace && workspace_bytes >= shape.bytes &&
+                                  reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+             "readout: product workspace too small or not 16-byte aligned");
+        ProductArgs p{m, n, k, a_scales, a_scale_stride, b_scales, b_scale_stride, b_tiles, out, out_stride, accumulate};
+        p.splits = shape.splits;
+        p.partials = static_cast<float*>(workspace);
+        if (out_dtype == MDSOAP_FLOAT32) run_product<float>(a, a_stride, b, b_stride, p, shape, sms, s);
+        else run_product<__nv_bfloat16>(a, a_stride, b, b_stride, p, shape, sms, s);
     });
 }
 
