@@ -96,6 +96,7 @@ __device__ __forceinline__ void store_row(OUT* p, int64_t left, const float (&f)
 
 constexpr int kPairTile = 256;
 constexpr int kPromote = 8;                    // warps that scale and add the partial products
+constexpr int kMine = kPairTile / (kPromote / 4);  // columns of one of their threads
 constexpr int kThreads = (kPromote + 4) * 32;  // a warp each for the copies and the matrix instructions, two to fill up
 // Registers: launched with 168 a thread; the last four warps give theirs up to 72
 // and the other eight take 216 (8 x 216 + 4 x 72 = 12 x 168).
@@ -115,6 +116,17 @@ struct PairShared {
     int gave_up;
     int issued;
 };
+
+constexpr int kStep = 16;  // columns that leave tensor memory at a time
+
+// acc + part x scale for a pair of columns.  Two scalar fmas: as one packed
+// fma.f32x2 the pairs needed as many register moves as it saved instructions.
+__device__ __forceinline__ uint64_t add_scaled(uint32_t x, uint32_t y, uint64_t scale, uint64_t acc) {
+    float m0, m1, a0, a1;
+    tc::split_pair(scale, m0, m1);
+    tc::split_pair(acc, a0, a1);
+    return tc::pair_of(fmaf(__uint_as_float(x), m0, a0), fmaf(__uint_as_float(y), m1, a1));
+}
 
 template <bool TILES, class OUT, Store STORE>
 __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_constant__ CUtensorMap map_a,
@@ -138,7 +150,7 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             bulk::barrier_init(&s.acc_full[i], 1);
-            bulk::barrier_init(&s.acc_empty[i], 2 * kPromote);
+            bulk::barrier_init(&s.acc_empty[i], 2 * kPromote);  // both CTAs' warps
         }
         bulk::barrier_init(&s.drained, 1);
         s.gave_up = 0;
@@ -162,14 +174,13 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
     if (warp >= kPromote) {
         tc::give_registers<kFewRegisters>();
         if (warp == kPromote && lane == 0) {
-            int count = 0;
+            int stage = 0, phase = 0, count = 0;
             bool good = true;
             for (int item = pair; item < items && good; item += pairs) {
                 const int m0 = item_m(item) + rank * kRows, n0 = item_n(item) + rank * kRows;
                 const int end = last_block(item);
                 for (int kb = first_block(item); kb < end; ++kb, ++count) {
-                    const int stage = count % kStages;
-                    if (!tc::wait(&s.empty[stage], (count / kStages & 1) ^ 1, gave_up)) {
+                    if (!tc::wait(&s.empty[stage], phase ^ 1, gave_up)) {
                         good = false;
                         break;
                     }
@@ -177,40 +188,45 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                     if (rank == 0) bulk::arrive_expect(&s.full[stage], 4 * kRows * kTileK);
                     tc::load_tile_pair(s.a[stage], &map_a, kb * kTileK, m0, full);
                     tc::load_tile_pair(s.b[stage], &map_b, kb * kTileK, n0, full);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
                 }
             }
             s.issued = count;
         } else if (warp == kPromote + 1 && lane == 0 && rank == 0) {
             constexpr uint32_t word = tc::instruction(kPairTile, kPairTile);
-            int count = 0;
-            for (int item = pair; item < items && !*gave_up; item += pairs) {
-                const int end = last_block(item);
-                for (int kb = first_block(item); kb < end; ++kb, ++count) {
-                    const int stage = count % kStages, buffer = count & 1;
-                    if (!tc::wait(&s.acc_empty[buffer], (count >> 1 & 1) ^ 1, gave_up)) break;
-                    if (!tc::wait(&s.full[stage], count / kStages & 1, gave_up)) break;
+            constexpr int kStep16 = kRows * kTileK / 16;  // descriptors count in units of 16 bytes
+            const uint64_t first_a = tc::operand(s.a[0]), first_b = tc::operand(s.b[0]);
+            int stage = 0, phase = 0, parity = 0, turn = 0;
+            bool good = true;
+            for (int item = pair; item < items && good; item += pairs) {
+                for (int left = last_block(item) - first_block(item); left > 0; --left) {
+                    const uint64_t a = first_a + stage * kStep16, b = first_b + stage * kStep16;
+                    const uint32_t d = tmem + parity * kPairTile;
+                    good = tc::wait(&s.full[stage], phase, gave_up) && tc::wait(&s.acc_empty[parity], turn ^ 1, gave_up);
+                    if (!good) break;
                     tc::fence_after();
-                    const uint64_t a = tc::operand(s.a[stage]), b = tc::operand(s.b[stage]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tc::mma<2>(tmem + buffer * kPairTile, a + 2 * k, b + 2 * k, word, k > 0);
+                    for (int k = 0; k < 4; ++k) tc::mma<2>(d, a + 2 * k, b + 2 * k, word, k > 0);
+                    tc::commit<2>(&s.acc_full[parity]);
                     tc::commit<2>(&s.empty[stage]);
-                    tc::commit<2>(&s.acc_full[buffer]);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                    parity ^= 1;
+                    turn ^= parity ^ 1;  // after every second block
                 }
             }
-            if (*gave_up) {  // matrix instructions in flight end before the tensor memory goes
+            if (!good) {  // matrix instructions in flight end before the tensor memory goes
                 tc::commit<2>(&s.drained);
                 bulk::wait(&s.drained, 0);
             }
         }
     } else {
         tc::take_registers<kManyRegisters>();
-        constexpr int kMine = kPairTile / 2;  // columns of one thread
         const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * kMine;
+        const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + half * kMine;
+        const uint32_t empty0 = tc::map_shared(&s.acc_empty[0], 0);
         const bool vec_a = p.a_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.a_scales) % 16 == 0;
         const bool vec_b = p.b_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.b_scales) % 16 == 0;
-        int count = 0;
+        int parity = 0, turn = 0;
         for (int item = pair; item < items; item += pairs) {
             const int m0 = item_m(item) + rank * kRows, n0 = item_n(item);
             const int begin = first_block(item), end = last_block(item);
@@ -224,59 +240,62 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < kMine / 2; ++i) acc[i] = 0;  // two zeros
             float4 next_a = scales4(sa, begin & ~3, end, vec_a), next_b = scales4(sb, begin & ~3, end, vec_b);
-            float4 scale = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int kb = begin; kb < end; ++kb, ++count) {
-                const int buffer = count & 1, group = kb >> 2 & 1;
-                if (kb == begin || (kb & 3) == 0) {  // the scales of four blocks at a time, loaded four blocks ahead
-                    if constexpr (TILES) {
-                        scale = make_float4(next_a.x * next_b.x, next_a.y * next_b.y, next_a.z * next_b.z,
-                                            next_a.w * next_b.w);
-                    } else {
-                        scale = next_a;
-                        s.b_scale[group][0][threadIdx.x] = next_b.x;
-                        s.b_scale[group][1][threadIdx.x] = next_b.y;
-                        s.b_scale[group][2][threadIdx.x] = next_b.z;
-                        s.b_scale[group][3][threadIdx.x] = next_b.w;
-                        asm volatile("bar.sync 1, %0;" ::"n"(kPromote * 32) : "memory");
-                    }
-                    next_a = scales4(sa, (kb & ~3) + 4, end, vec_a);
-                    next_b = scales4(sb, (kb & ~3) + 4, end, vec_b);
+            // four blocks a turn: their scales were loaded one turn ahead
+            for (int first = begin & ~3; first < end; first += 4) {
+                float scale[4] = {next_a.x, next_a.y, next_a.z, next_a.w};
+                const int group = first >> 2 & 1;
+                if constexpr (TILES) {
+                    scale[0] *= next_b.x, scale[1] *= next_b.y, scale[2] *= next_b.z, scale[3] *= next_b.w;
+                } else {
+                    s.b_scale[group][0][threadIdx.x] = next_b.x;
+                    s.b_scale[group][1][threadIdx.x] = next_b.y;
+                    s.b_scale[group][2][threadIdx.x] = next_b.z;
+                    s.b_scale[group][3][threadIdx.x] = next_b.w;
+                    // the four warps that share a half of the columns
+                    asm volatile("bar.sync %0, %1;" ::"r"(1 + half), "n"(kRows) : "memory");
                 }
-                const float mine = pick(scale, kb & 3);
-                const uint64_t mine2 = tc::pair_of(mine, mine);
-                tc::wait(&s.acc_full[buffer], count >> 1 & 1, gave_up);
-                __syncwarp();
-                tc::fence_after();
+                next_a = scales4(sa, first + 4, end, vec_a);
+                next_b = scales4(sb, first + 4, end, vec_b);
 #pragma unroll
-                for (int c = 0; c < kMine; c += 32) {
-                    uint32_t part[32];
-                    tc::load32(from + buffer * kPairTile + c, part);
-                    tc::wait_loads();
-                    if (c + 32 == kMine) {
-                        tc::fence_before();
-                        __syncwarp();
-                        if (lane == 0) tc::arrive_at(tc::map_shared(&s.acc_empty[buffer], 0));
-                    }
-                    if constexpr (TILES) {
+                for (int j = 0; j < 4; ++j) {
+                    if (first + j < begin || first + j >= end) continue;
+                    const uint64_t mine2 = tc::pair_of(scale[j], scale[j]);
+                    const uint32_t from = lanes + parity * kPairTile;
+                    const ulonglong2* sb2 =
+                        reinterpret_cast<const ulonglong2*>(&s.b_scale[TILES ? 0 : group][j][TILES ? 0 : half * kMine]);
+                    tc::wait(&s.acc_full[parity], turn, gave_up);
+                    __syncwarp();
+                    tc::fence_after();
+                    // the next columns leave tensor memory while these are added
+                    uint32_t part[2][kStep];
+                    tc::load(from, part[0]);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            acc[c / 2 + i] = tc::fma2(
-                                tc::pair_of(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])), mine2,
-                                acc[c / 2 + i]);
-                    } else {
-                        const ulonglong2* sb2 =
-                            reinterpret_cast<const ulonglong2*>(&s.b_scale[group][kb & 3][half * kMine + c]);
+                    for (int c = 0; c < kMine; c += kStep) {
+                        tc::wait_loads();
+                        if (c + kStep < kMine) {
+                            tc::load(from + c + kStep, part[(c / kStep + 1) & 1]);
+                        } else {
+                            tc::fence_before();
+                            __syncwarp();
+                            if (lane == 0) tc::arrive_at(empty0 + parity * (uint32_t)sizeof(uint64_t));
+                        }
+                        const uint32_t(&now)[kStep] = part[c / kStep & 1];
+                        if constexpr (TILES) {
 #pragma unroll
-                        for (int i = 0; i < 16; i += 2) {
-                            const ulonglong2 q = sb2[i / 2];
-                            acc[c / 2 + i] = tc::fma2(
-                                tc::pair_of(__uint_as_float(part[2 * i]), __uint_as_float(part[2 * i + 1])),
-                                tc::mul2(mine2, q.x), acc[c / 2 + i]);
-                            acc[c / 2 + i + 1] = tc::fma2(
-                                tc::pair_of(__uint_as_float(part[2 * i + 2]), __uint_as_float(part[2 * i + 3])),
-                                tc::mul2(mine2, q.y), acc[c / 2 + i + 1]);
+                            for (int i = 0; i < kStep / 2; ++i)
+                                acc[c / 2 + i] = add_scaled(now[2 * i], now[2 * i + 1], mine2, acc[c / 2 + i]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < kStep / 2; i += 2) {
+                                const ulonglong2 q = sb2[(c + 2 * i) / 4];
+                                acc[c / 2 + i] = add_scaled(now[2 * i], now[2 * i + 1], tc::mul2(mine2, q.x), acc[c / 2 + i]);
+                                acc[c / 2 + i + 1] =
+                                    add_scaled(now[2 * i + 2], now[2 * i + 3], tc::mul2(mine2, q.y), acc[c / 2 + i + 1]);
+                            }
                         }
                     }
+                    parity ^= 1;
+                    turn ^= parity ^ 1;
                 }
             }
             if (*gave_up) break;

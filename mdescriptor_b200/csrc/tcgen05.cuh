@@ -181,7 +181,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sy
 // Waits for a barrier phase; false (and *gave_up set) once a second has passed
 // or another thread of the CTA gave up.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-    if (bulk::try_wait(bar, parity)) return true;
+    if (bulk::try_wait(bar, parity) || bulk::try_wait(bar, parity)) return true;
     const uint64_t start = bulk::global_ns();
     while (!bulk::try_wait(bar, parity)) {
         if (*gave_up) return false;
