@@ -35,7 +35,8 @@ struct RowArgs {
     int64_t scale_stride;
 };
 
-// One row by one warp (CTA_ROW false) or by the CTA's warps together.
+// One row by one warp (CTA_ROW false) or by the CTA's warps together, a block
+// of 128 at a time, four elements a lane.
 //
 // s = x + r; rstd = (mean s^2 + eps)^-1/2; y = s rstd w.  In 8 bits the factor
 // rstd is constant in the row, so it cancels from the codes 448 z / max|z| of
@@ -44,10 +45,98 @@ struct RowArgs {
 // shared memory, one float a block).  Nothing of the row is held or read twice.
 // Bound by HBM: x and r once in, sum and codes once out.
 template <class T, bool CTA_ROW, Rows MODE>
+struct RowPass {
+    using Word = typename Quad<T>::Word;
+    static constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+    const RowArgs<T>& a;
+    const T* x;
+    const T* r;  // null without a residual
+    T* sum;      // null where it is not wanted
+    uint8_t* codes;
+    float* top;
+    int64_t width;
+    uintptr_t x_begin, x_end, r_begin, r_end;
+    float total;
+
+    // One block from its words.  FULL: all 128 columns exist and rows are aligned to words.
+    template <bool FULL>
+    __device__ __forceinline__ void block(int64_t col, const Word& wx, const Word& wr) {
+        const int lane = threadIdx.x & 31;
+        float4 s = unpack4<T>(wx);
+        if (r) {
+            const float4 f = unpack4<T>(wr);
+            s.x += f.x, s.y += f.y, s.z += f.z, s.w += f.w;
+        }
+        if constexpr (MODE != Rows::Quantize) {
+            total = fmaf(s.x, s.x, fmaf(s.y, s.y, fmaf(s.z, s.z, fmaf(s.w, s.w, total))));
+            if (sum) {
+                if constexpr (FULL) *reinterpret_cast<Word*>(sum + col) = pack4<T>(s);
+                else store_quad(sum, col, width, pack4<T>(s));
+            }
+        }
+        if constexpr (MODE != Rows::NormWide) {
+            float4 z = s, rest = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (a.col_factor) {
+                float w[4];
+                load_vector<4>(a.col_factor, col, width, w);
+                z = make_float4(s.x * w[0], s.y * w[1], s.z * w[2], s.w * w[3]);
+                rest = make_float4(fmaf(s.x, w[0], -z.x), fmaf(s.y, w[1], -z.y), fmaf(s.z, w[2], -z.z),
+                                   fmaf(s.w, w[3], -z.w));
+            }
+            const float most = warp_larger(larger(larger(larger(fabsf(z.x), z.y), z.z), z.w));
+            const Factor factor(most);
+            if (FULL || col < width) {  // the pitch covers a quad's padding
+                if (lane == 0) top[col / kBlock] = most;
+                *reinterpret_cast<uint32_t*>(codes + col) =
+                    codes4(factor(z.x, rest.x), factor(z.y, rest.y), factor(z.z, rest.z), factor(z.w, rest.w));
+            }
+        }
+    }
+
+    // kAhead blocks from `b` on, their words loaded first.
+    template <bool ALIGNED>
+    __device__ __forceinline__ void several(int b, int step) {
+        const int lane = threadIdx.x & 31;
+        Word wx[kAhead], wr[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int64_t col = (int64_t)(b + i * step) * kBlock + lane * 4;
+            wx[i] = ALIGNED ? __ldg(reinterpret_cast<const Word*>(x + col)) : load_split(x + col);
+            wr[i] = !r ? Word{} : ALIGNED ? __ldg(reinterpret_cast<const Word*>(r + col)) : load_split(r + col);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            block<ALIGNED>((int64_t)(b + i * step) * kBlock + lane * 4, wx[i], wr[i]);
+    }
+
+    // Whether the aligned words around columns [0, columns) of a row lie inside its matrix.
+    __device__ __forceinline__ bool inside(const T* row, int64_t columns, uintptr_t begin, uintptr_t end) const {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row), shift = at % sizeof(Word);
+        return shift == 0 || (at - shift >= begin && at - shift + columns * sizeof(T) + sizeof(Word) <= end);
+    }
+
+    // The warp's blocks: kAhead of them under way at a time.
+    __device__ __forceinline__ void run(int first, int step) {
+        const int lane = threadIdx.x & 31;
+        const int full = (int)(width / kBlock);
+        int b = first;
+        if (quads_aligned(x) && (!r || quads_aligned(r)) && (!sum || quads_aligned(sum))) {
+            for (; b + (kAhead - 1) * step < full; b += kAhead * step) several<true>(b, step);
+        } else if (inside(x, (int64_t)full * kBlock, x_begin, x_end) &&
+                   (!r || inside(r, (int64_t)full * kBlock, r_begin, r_end))) {
+            for (; b + (kAhead - 1) * step < full; b += kAhead * step) several<false>(b, step);
+        }
+        for (; (int64_t)b * kBlock < width; b += step) {
+            const int64_t col = (int64_t)b * kBlock + lane * 4;
+            const Word wx = load_quad(x, col, width, x_begin, x_end);
+            const Word wr = r ? load_quad(r, col, width, r_begin, r_end) : Word{};
+            block<false>(col, wx, wr);
+        }
+    }
+};
+
+template <class T, bool CTA_ROW, Rows MODE>
 __global__ __launch_bounds__(kRowWarps * 32) void rows_kernel(const __grid_constant__ RowArgs<T> a) {
-    constexpr int N = kUnit<T>;
-    constexpr int kChunk = 32 * N;            // columns a warp takes at a time
-    constexpr int kLanes = kBlock / N;        // lanes of one block of 128: 16 or 32
     extern __shared__ float s_top[];
     __shared__ float s_sum[kRowWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -55,57 +144,25 @@ __global__ __launch_bounds__(kRowWarps * 32) void rows_kernel(const __grid_const
     if (row >= a.x.rows) return;  // never with CTA_ROW, whose warps meet below
     const int64_t width = a.x.width;
     const int64_t nblocks = (width + kBlock - 1) / kBlock;
-    float* const top = s_top + (CTA_ROW ? 0 : warp * nblocks);
-    const MatrixIn<T> r{a.residual, a.x.rows, width, a.residual_stride};
-    const int64_t step = (CTA_ROW ? kRowWarps : 1) * (int64_t)kChunk;
-    const int64_t first = (CTA_ROW ? warp * (int64_t)kChunk : 0) + lane * N;
-
-    float total = 0.0f;
-    for (int64_t col = first; col - lane * N < width; col += step) {
-        float s[N];
-        unpack<T>(a.x.unit(row, col), s);
-        if (a.residual) {
-            float f[N];
-            unpack<T>(r.unit(row, col), f);
-#pragma unroll
-            for (int i = 0; i < N; ++i) s[i] += f[i];
-        }
-        if constexpr (MODE != Rows::Quantize) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) total = fmaf(s[i], s[i], total);
-            if (a.sum) store_unit(a.sum + row * a.sum_stride, col, width, pack<T>(s));
-        }
-        if constexpr (MODE != Rows::NormWide) {
-            if (a.col_factor) {
-                float w[N];
-                load_vector<N>(a.col_factor, col, width, w);
-#pragma unroll
-                for (int i = 0; i < N; ++i) s[i] *= w[i];
-            }
-            uint32_t most = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) most = max(most, magnitude(s[i]));
-#pragma unroll
-            for (int d = kLanes / 2; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-            const float block_top = __uint_as_float(most);
-            if (col < width) {
-                if (lane % kLanes == 0) top[col / kBlock] = block_top;
-                const Factor factor(block_top);
-                uint8_t* out = a.codes + row * a.code_stride + col;  // the pitch covers the unit's padding
-                if constexpr (N == 8) {
-                    *reinterpret_cast<uint2*>(out) =
-                        make_uint2(codes4(factor(s[0]), factor(s[1]), factor(s[2]), factor(s[3])),
-                                   codes4(factor(s[4]), factor(s[5]), factor(s[6]), factor(s[7])));
-                } else {
-                    *reinterpret_cast<uint32_t*>(out) = codes4(factor(s[0]), factor(s[1]), factor(s[2]), factor(s[3]));
-                }
-            }
-        }
-    }
+    const auto span_end = [&](const T* p, int64_t stride) {
+        return reinterpret_cast<uintptr_t>(p + (a.x.rows - 1) * stride + width);
+    };
+    RowPass<T, CTA_ROW, MODE> pass{a,
+                                   a.x.data + row * a.x.stride,
+                                   a.residual ? a.residual + row * a.residual_stride : nullptr,
+                                   MODE != Rows::Quantize && a.sum ? a.sum + row * a.sum_stride : nullptr,
+                                   a.codes + row * a.code_stride,
+                                   s_top + (CTA_ROW ? 0 : warp * nblocks),
+                                   width,
+                                   reinterpret_cast<uintptr_t>(a.x.data), span_end(a.x.data, a.x.stride),
+                                   reinterpret_cast<uintptr_t>(a.residual), span_end(a.residual, a.residual_stride),
+                                   0.0f};
+    const int first = CTA_ROW ? warp : 0, step = CTA_ROW ? kRowWarps : 1;
+    pass.run(first, step);
 
     float row_scale = 1.0f;
     if constexpr (MODE != Rows::Quantize) {
-        total = warp_sum(total);
+        float total = warp_sum(pass.total);
         if constexpr (CTA_ROW) {
             if (lane == 0) s_sum[warp] = total;
             __syncthreads();
@@ -116,32 +173,29 @@ __global__ __launch_bounds__(kRowWarps * 32) void rows_kernel(const __grid_const
         row_scale = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(total, (float)width) + a.eps));
         if (a.rstd && lane == 0 && (!CTA_ROW || warp == 0)) a.rstd[row] = row_scale;
     } else if (a.row_factor) {
-        row_scale = a.row_factor[row];
+        row_scale = a.row_factor[row];  // a negative one shows in the scales' sign
     }
     if constexpr (CTA_ROW) __syncthreads();
     __syncwarp();
 
     if constexpr (MODE == Rows::NormWide) {
-        for (int64_t col = first; col - lane * N < width; col += step) {
-            float s[N], w[N];
-            unpack<T>(a.x.unit(row, col), s);
-            if (a.residual) {
-                float f[N];
-                unpack<T>(r.unit(row, col), f);
-#pragma unroll
-                for (int i = 0; i < N; ++i) s[i] += f[i];
+        for (int64_t b = first; b < nblocks; b += step) {
+            const int64_t col = b * kBlock + lane * 4;
+            float4 s = unpack4<T>(load_quad(pass.x, col, width, pass.x_begin, pass.x_end));
+            if (pass.r) {
+                const float4 f = unpack4<T>(load_quad(pass.r, col, width, pass.r_begin, pass.r_end));
+                s.x += f.x, s.y += f.y, s.z += f.z, s.w += f.w;
             }
-            load_vector<N>(a.col_factor, col, width, w);
-#pragma unroll
-            for (int i = 0; i < N; ++i) s[i] = s[i] * row_scale * w[i];
-            store_unit(a.wide + row * a.wide_stride, col, width, pack<T>(s));
+            float w[4];
+            load_vector<4>(a.col_factor, col, width, w);
+            store_quad(a.wide + row * a.wide_stride, col, width,
+                       pack4<T>(make_float4(s.x * row_scale * w[0], s.y * row_scale * w[1], s.z * row_scale * w[2],
+                                            s.w * row_scale * w[3])));
         }
     } else {
-        // A negative row factor turns the signs of the codes, which are written
-        // already: the quantiser takes it through its scale's sign instead.
         const int at = CTA_ROW ? threadIdx.x : lane;
         for (int64_t b = at; b < nblocks; b += CTA_ROW ? kRowWarps * 32 : 32)
-            a.scales[row * a.scale_stride + b] = scale_of(top[b]) * row_scale;
+            a.scales[row * a.scale_stride + b] = scale_of(pass.top[b]) * row_scale;
     }
 }
 
@@ -175,12 +229,17 @@ void launch_rows(const RowArgs<T>& a, int sms, cudaStream_t stream) {
 //
 // c = sum_d dy w s;  ds = rstd w dy - s rstd^3 c / D (+ dsum);  dw = sum_t dy s rstd.
 //
-// A CTA of G threads takes rows b, b + grid, ...: each thread owns the same NU
-// units of every row, so the row stays in registers between the sum c and the
-// result, and the weight's gradient adds up in registers over the CTA's rows.
-// The partial sums of all CTAs go to the workspace and are added in CTA order
-// by a second kernel: the same bits on every run.  Bound by HBM: dy, s, dsum
-// once in, ds once out.
+// A CTA takes rows b, b + grid, ...: each thread owns the same NU units of 16
+// bytes of every row, so the row stays in registers between the sum c and the
+// result (the next row's units already under way), and the weight's gradient
+// adds up in registers over the CTA's rows.  The partial sums of all CTAs go to
+// the workspace and are added in CTA order by a second kernel: the same bits on
+// every run.  Bound by HBM: dy, s, dsum once in, ds once out.
+//
+// ALIKE: the matrices' rows sit alike relative to 16 bytes.  With an odd width
+// the rows' alignment repeats every eight rows at most; the grid is a multiple of
+// that, so all rows of a CTA are aligned alike and its units are whole 16-byte
+// words of all of them (the first and last of a row partly another row's).
 template <class T>
 struct NormBackwardArgs {
     MatrixIn<T> dy, s;
@@ -195,65 +254,96 @@ struct NormBackwardArgs {
     float* dots;  // wide rows only: c of each row
 };
 
-template <int G>
+// The sum over the CTA's warps; `scratch` holds one float a warp.
 __device__ __forceinline__ float cta_sum(float x, float* scratch) {
     x = warp_sum(x);
-    if constexpr (G == 32) return x;
+    if (blockDim.x == 32) return x;
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
     float total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < G / 32; ++w) total += scratch[w];
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) total += scratch[w];
     return total;
 }
 
-template <class T, int G, int NU>
-__global__ __launch_bounds__(G) void norm_backward_kernel(const __grid_constant__ NormBackwardArgs<T> a) {
+template <class T, int NU, bool ALIKE>
+__global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(const __grid_constant__ NormBackwardArgs<T> a) {
     constexpr int N = kUnit<T>;
-    __shared__ float scratch[2][G / 32];
-    const int64_t width = a.s.width;
-    const MatrixIn<T> dsum{a.dsum, a.s.rows, width, a.dsum_stride};
-    float w[NU][N], dw[NU][N];
+    constexpr bool kAhead = NU <= 2;  // the next row's units are loaded a row ahead; the weight stays in registers
+    __shared__ float scratch[2][16];
+    const int width = (int)a.s.width, threads = blockDim.x;
+    const MatrixIn<T> dsum{a.dsum, a.s.rows, a.s.width, a.dsum_stride};
+    const int64_t first = blockIdx.x;
+    const int before = ALIKE ? (int)(reinterpret_cast<uintptr_t>(a.s.data + first * a.s.stride) % 16 / sizeof(T)) : 0;
+
+    int col[NU];
+    bool whole[NU];
+    float w[kAhead ? NU : 1][N], dw[NU][N];
+    const auto weight_of = [&](int u, float (&f)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = col[u] + i >= 0 && col[u] + i < width ? __ldg(a.weight + col[u] + i) : 0.0f;
+    };
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        load_vector<N>(a.weight, ((int64_t)u * G + threadIdx.x) * N, width, w[u]);
+        col[u] = (u * threads + threadIdx.x) * N - before;
+        whole[u] = col[u] >= 0 && col[u] + N <= width;
+        if constexpr (kAhead) weight_of(u, w[u]);
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[u][i] = 0.0f;
     }
+    const auto load = [&](const MatrixIn<T>& m, int64_t row, int u) {
+        if constexpr (!ALIKE) return m.unit(row, col[u]);
+        const T* p = m.data + row * m.stride + col[u];
+        if (whole[u]) return __ldg(reinterpret_cast<const uint4*>(p));
+        uint4 q = make_uint4(0, 0, 0, 0);
+        T* t = reinterpret_cast<T*>(&q);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col[u] + i >= 0 && col[u] + i < width) t[i] = p[i];
+        return q;
+    };
+
     const float inv_width = __fdiv_rn(1.0f, (float)width);
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < a.s.rows; row += gridDim.x, turn ^= 1) {
-        uint4 qdy[NU], qs[NU], qd[NU];
+    uint4 qdy[NU], qs[NU], qd[NU], next_dy[NU], next_s[NU], next_d[NU];
+    float rstd = 0.0f, next_rstd = 0.0f;
+    const auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int64_t col = ((int64_t)u * G + threadIdx.x) * N;
-            qdy[u] = a.dy.unit(row, col);
-            qs[u] = a.s.unit(row, col);
-            if (a.dsum) qd[u] = dsum.unit(row, col);
+            next_dy[u] = load(a.dy, row, u);
+            next_s[u] = load(a.s, row, u);
+            if (a.dsum) next_d[u] = load(dsum, row, u);
         }
-        const float rstd = a.rstd[row];
+        next_rstd = a.rstd[row];
+    };
+    if (kAhead && first < a.s.rows) fetch(first);
+    int turn = 0;
+    for (int64_t row = first; row < a.s.rows; row += gridDim.x, turn ^= 1) {
+        if (!kAhead) fetch(row);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) qdy[u] = next_dy[u], qs[u] = next_s[u], qd[u] = next_d[u];
+        rstd = next_rstd;
+        if (kAhead && row + gridDim.x < a.s.rows) fetch(row + gridDim.x);
         float c = 0.0f;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            float dy[N], s[N];
+            float dy[N], s[N], g[N];
             unpack<T>(qdy[u], dy);
             unpack<T>(qs[u], s);
+            if constexpr (!kAhead) weight_of(u, g);
 #pragma unroll
-            for (int i = 0; i < N; ++i) c = fmaf(dy[i] * w[u][i], s[i], c);
+            for (int i = 0; i < N; ++i) c = fmaf(dy[i] * (kAhead ? w[kAhead ? u : 0][i] : g[i]), s[i], c);
         }
         // two scratch rows in turn: a warp may be one row ahead of another, never two
-        c = cta_sum<G>(c, scratch[turn]) * inv_width * rstd * rstd;
+        c = cta_sum(c, scratch[turn]) * inv_width * rstd * rstd;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int64_t col = ((int64_t)u * G + threadIdx.x) * N;
-            float dy[N], s[N], out[N];
+            float dy[N], s[N], out[N], g[N];
             unpack<T>(qdy[u], dy);
             unpack<T>(qs[u], s);
+            if constexpr (!kAhead) weight_of(u, g);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float hat = s[i] * rstd;
-                dw[u][i] = fmaf(dy[i], hat, dw[u][i]);
-                out[i] = rstd * fmaf(-s[i], c, dy[i] * w[u][i]);
+                dw[u][i] = fmaf(dy[i], s[i] * rstd, dw[u][i]);
+                out[i] = rstd * fmaf(-s[i], c, dy[i] * (kAhead ? w[kAhead ? u : 0][i] : g[i]));
             }
             if (a.dsum) {
                 float d[N];
@@ -261,18 +351,27 @@ __global__ __launch_bounds__(G) void norm_backward_kernel(const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < N; ++i) out[i] += d[i];
             }
-            store_unit(a.dx + row * a.dx_stride, col, width, pack<T>(out));
+            if constexpr (ALIKE) {
+                T* p = a.dx + row * a.dx_stride + col[u];
+                const uint4 q = pack<T>(out);
+                if (whole[u]) {
+                    *reinterpret_cast<uint4*>(p) = q;
+                } else {
+                    const T* t = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (col[u] + i >= 0 && col[u] + i < width) p[i] = t[i];
+                }
+            } else {
+                store_unit(a.dx + row * a.dx_stride, col[u], width, pack<T>(out));
+            }
         }
     }
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-        const int64_t col = ((int64_t)u * G + threadIdx.x) * N;
-        if (col < width) {  // the pitch covers a whole unit
-            float4* p = reinterpret_cast<float4*>(a.partial + blockIdx.x * a.pitch + col);
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int i = 0; i < N; i += 4) p[i / 4] = make_float4(dw[u][i], dw[u][i + 1], dw[u][i + 2], dw[u][i + 3]);
-        }
-    }
+        for (int i = 0; i < N; ++i)
+            if (col[u] + i >= 0 && col[u] + i < width) a.partial[blockIdx.x * a.pitch + col[u] + i] = dw[u][i];
 }
 
 // Rows too wide for one CTA's registers: c of each row first ...
@@ -290,7 +389,7 @@ __global__ __launch_bounds__(256) void norm_dots_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < N; ++i) c = fmaf(dy[i] * w[i], s[i], c);
     }
-    c = cta_sum<256>(c, scratch);
+    c = cta_sum(c, scratch);
     if (threadIdx.x == 0) a.dots[row] = c;
 }
 
@@ -365,48 +464,46 @@ struct BackwardShape {
     size_t bytes;
 };
 
-// Threads and units so that a row fits a CTA's registers (units x 16 bytes a
-// thread); grids of about 2048 threads an SM.
+// Threads and units so that a row (and the word that an odd start adds) fits a
+// CTA's registers, and a grid that the SMs hold at once: by registers, 64 a
+// thread with one unit and 128 with more.
 BackwardShape backward_shape(int64_t rows, int64_t width, int unit, int sms) {
     BackwardShape s{};
     s.pitch = (width + 7) / 8 * 8;
-    const int64_t units = (width + unit - 1) / unit;
-    if (units <= 32) s.threads = 32, s.units = 1;
-    else if (units <= 64) s.threads = 64, s.units = 1;
-    else if (units <= 128) s.threads = 128, s.units = 1;
-    else if (units <= 256) s.threads = 128, s.units = 2;
-    else if (units <= 512) s.threads = 256, s.units = 2;
-    else if (units <= 1024) s.threads = 512, s.units = 2;
-    else if (units <= 2048) s.threads = 512, s.units = 4;
-    const int64_t resident = s.threads ? std::min(1024 / s.threads, 16) : 8;
-    s.grid = std::max<int64_t>(1, std::min<int64_t>(rows, resident * sms));
+    const int64_t units = (width + unit - 1) / unit + 1;
+    s.units = units <= 512 ? 1 : units <= 1024 ? 2 : 4;
+    if (units <= 2048) s.threads = (int)((units + s.units * 32 - 1) / (s.units * 32) * 32);
+    const int64_t resident =
+        s.threads ? std::max<int64_t>(1, std::min<int64_t>((s.units == 1 ? 1024 : 512) / s.threads, 16)) : 8;
+    // a multiple of eight, so that the rows of one CTA are aligned alike; or a CTA a row
+    s.grid = std::max<int64_t>(1, std::min<int64_t>(rows, std::max<int64_t>(8, resident * sms / 8 * 8)));
     s.bytes = (size_t)s.grid * s.pitch * sizeof(float) + (s.threads ? 0 : (size_t)rows * sizeof(float));
     return s;
 }
 
-template <class T, int G, int NU>
-void launch_backward(const NormBackwardArgs<T>& a, const BackwardShape& s, cudaStream_t stream) {
-    norm_backward_kernel<T, G, NU><<<(unsigned)s.grid, G, 0, stream>>>(a);
+// Whether rows of a matrix sit like those of `s` relative to 16 bytes.
+template <class T>
+bool alike(const T* p, int64_t stride, const MatrixIn<T>& s) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == reinterpret_cast<uintptr_t>(s.data) % 16 &&
+           (stride - s.stride) * (int64_t)sizeof(T) % 16 == 0;
 }
 
 template <class T>
 void norm_backward(NormBackwardArgs<T> a, float* dweight, const BackwardShape& s, cudaStream_t stream) {
-    const int key = s.threads * 8 + s.units;
-    switch (key) {
-        case 32 * 8 + 1: launch_backward<T, 32, 1>(a, s, stream); break;
-        case 64 * 8 + 1: launch_backward<T, 64, 1>(a, s, stream); break;
-        case 128 * 8 + 1: launch_backward<T, 128, 1>(a, s, stream); break;
-        case 128 * 8 + 2: launch_backward<T, 128, 2>(a, s, stream); break;
-        case 256 * 8 + 2: launch_backward<T, 256, 2>(a, s, stream); break;
-        case 512 * 8 + 2: launch_backward<T, 512, 2>(a, s, stream); break;
-        case 512 * 8 + 4: launch_backward<T, 512, 4>(a, s, stream); break;
-        default: {
-            a.dots = a.partial + s.grid * s.pitch;
-            norm_dots_kernel<T><<<(unsigned)a.s.rows, 256, 0, stream>>>(a);
-            check(cudaGetLastError(), "norm gradient launch");
-            const int64_t stripes = (a.s.width + 256 * kUnit<T> - 1) / (256 * kUnit<T>);
-            norm_stripes_kernel<T><<<dim3((unsigned)s.grid, (unsigned)stripes), 256, 0, stream>>>(a);
-        }
+    if (s.threads) {
+        const bool same = alike(a.dy.data, a.dy.stride, a.s) && alike(static_cast<const T*>(a.dx), a.dx_stride, a.s) &&
+                          (!a.dsum || alike(a.dsum, a.dsum_stride, a.s));
+        const auto kernel = s.units == 1   ? (same ? norm_backward_kernel<T, 1, true> : norm_backward_kernel<T, 1, false>)
+                            : s.units == 2 ? (same ? norm_backward_kernel<T, 2, true> : norm_backward_kernel<T, 2, false>)
+                                           : (same ? norm_backward_kernel<T, 4, true> : norm_backward_kernel<T, 4, false>);
+        kernel<<<(unsigned)s.grid, s.threads, 0, stream>>>(a);
+    } else {
+        a.dots = a.partial + s.grid * s.pitch;
+        norm_dots_kernel<T><<<(unsigned)a.s.rows, 256, 0, stream>>>(a);
+        check(cudaGetLastError(), "norm gradient launch");
+        const int64_t stripes = (a.s.width + 256 * kUnit<T> - 1) / (256 * kUnit<T>);
+        need(stripes <= 65535, "readout: norm gradient too wide");
+        norm_stripes_kernel<T><<<dim3((unsigned)s.grid, (unsigned)stripes), 256, 0, stream>>>(a);
     }
     check(cudaGetLastError(), "norm gradient launch");
     column_sum_kernel<<<(unsigned)((a.s.width + 31) / 32), 256, 0, stream>>>(a.partial, s.pitch, (int)s.grid, a.s.width,
@@ -432,173 +529,144 @@ struct TileArgs {
 };
 
 // One CTA a tile of 128 rows x 128 columns, read once into registers: warp w
-// holds rows 16 w .. 16 w + 15, a lane kUnit neighbouring columns of each of
-// its rows.  Blocks along the rows are reduced inside a (half) warp, blocks
-// along the columns over the warps through shared memory.  The transposed
-// codes meet in a 16 KB tile of shared memory whose 8-byte pieces are placed
-// at piece ^ (column / unit), so that both the stores of consecutive rows and
-// the 16-byte reads along them are free of bank conflicts.
+// holds rows 16 w .. 16 w + 15, a lane four neighbouring columns of each.
+// Blocks along the rows are reduced inside the warp, blocks along the columns
+// over the warps through shared memory.  The transposed codes meet in a 16 KB
+// tile of shared memory whose 16-byte pieces (16 rows of a column) are placed at
+// piece ^ column / 4, so that both the stores of a lane's four columns and the
+// reads along a column are free of bank conflicts.
 // TILES: one scale for the whole tile, in both directions.
 // Bound by HBM: every element once in, one byte out a direction.
-template <class T, bool ROWS, bool COLS, bool TILES>
-__global__ __launch_bounds__(256) void tile_kernel(const __grid_constant__ TileArgs<T> a) {
-    constexpr int N = kUnit<T>;
-    constexpr int kLanes = kBlock / N;          // lanes of one row of the tile: 16 or 32
-    constexpr int kPart = 32 / kLanes;          // rows a warp reads at a time
-    constexpr int kMine = 16 / kPart;           // rows of one lane, consecutive
-    __shared__ __align__(16) uint8_t s_codes[COLS ? 128 * 128 : 16];
-    __shared__ uint32_t s_top[8][128];
+template <class T, bool ROWS, bool TILES>
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const __grid_constant__ TileArgs<T> a) {
+    using Word = typename Quad<T>::Word;
+    __shared__ __align__(16) uint8_t s_codes[128 * 128];
+    __shared__ __align__(16) float s_top[8][128];
+    __shared__ float s_factor[128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tile_row = (int64_t)blockIdx.y * 128, tile_col = (int64_t)blockIdx.x * 128;
-    const int row0 = warp * 16 + lane / kLanes * kMine;
-    const int col0 = lane % kLanes * N;
-    const int64_t rows = a.x.rows, width = a.x.width;
+    const int row0 = warp * 16, col0 = lane * 4;
+    const int64_t rows = a.x.rows, width = a.x.width, col = tile_col + col0;
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(a.x.data);
+    const uintptr_t end = reinterpret_cast<uintptr_t>(a.x.data + (rows - 1) * a.x.stride + width);
 
-    uint4 raw[kMine];
+    Word raw[16];
+    const T* from = a.x.data + (tile_row + row0) * a.x.stride;
+    if (tile_row + 128 <= rows && tile_col + 128 <= width && quads_aligned(a.x.data) &&
+        a.x.stride * sizeof(T) % sizeof(Word) == 0) {
 #pragma unroll
-    for (int i = 0; i < kMine; ++i)
-        raw[i] = tile_row + row0 + i < rows ? a.x.unit(tile_row + row0 + i, tile_col + col0) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 16; ++i) raw[i] = __ldg(reinterpret_cast<const Word*>(from + i * a.x.stride + col));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            raw[i] = tile_row + row0 + i < rows ? load_quad(from + i * a.x.stride, col, width, begin, end) : Word{};
+    }
+    // along a column its own factor cancels, only the rows' factors enter the codes, and the other way round
+    const bool row_factor = !TILES && a.row_factor, col_factor = ROWS && !TILES && a.col_factor;
+    if (row_factor) {
+        if (threadIdx.x < 128)
+            s_factor[threadIdx.x] = tile_row + threadIdx.x < rows ? a.row_factor[tile_row + threadIdx.x] : 0.0f;
+        __syncthreads();
+    }
+    float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (col_factor) load_vector<4>(a.col_factor, col, width, g);
 
-    float g[N];
-    if (!TILES && ROWS && a.col_factor) load_vector<N>(a.col_factor, tile_col + col0, width, g);
-
-    uint32_t col_top[N];
+    float4 col_top = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) col_top[j] = 0;
-    uint32_t all_top = 0;
-#pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        float z[N];
-        unpack<T>(raw[i], z);
+    for (int i = 0; i < 16; ++i) {
+        const float4 x = unpack4<T>(raw[i]);
         const int64_t row = tile_row + row0 + i;
-        if constexpr (COLS && !TILES) {
-            // along a column its own factor cancels: only the rows' factors enter the codes
-            const float f = a.row_factor && row < rows ? a.row_factor[row] : 1.0f;
-#pragma unroll
-            for (int j = 0; j < N; ++j) col_top[j] = max(col_top[j], magnitude(z[j] * f));
-        }
-        if constexpr (TILES) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) all_top = max(all_top, magnitude(z[j]));
-        }
+        const float f = row_factor ? s_factor[row0 + i] : 1.0f;
+        col_top = make_float4(larger(col_top.x, x.x * f), larger(col_top.y, x.y * f), larger(col_top.z, x.z * f),
+                              larger(col_top.w, x.w * f));
         if constexpr (ROWS && !TILES) {
-            uint32_t most = 0;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                if (a.col_factor) z[j] *= g[j];
-                most = max(most, magnitude(z[j]));
-            }
-#pragma unroll
-            for (int d = kLanes / 2; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
-            const float top = __uint_as_float(most);
-            const Factor factor(top);
-            if (row < rows && tile_col + col0 < width) {
-                uint8_t* out = a.codes + row * a.code_stride + tile_col + col0;
-                if constexpr (N == 8)
-                    *reinterpret_cast<uint2*>(out) =
-                        make_uint2(codes4(factor(z[0]), factor(z[1]), factor(z[2]), factor(z[3])),
-                                   codes4(factor(z[4]), factor(z[5]), factor(z[6]), factor(z[7])));
-                else
-                    *reinterpret_cast<uint32_t*>(out) = codes4(factor(z[0]), factor(z[1]), factor(z[2]), factor(z[3]));
-                if (lane % kLanes == 0)
-                    a.scales[row * a.scale_stride + blockIdx.x] =
-                        scale_of(top) * (a.row_factor ? a.row_factor[row] : 1.0f);
+            const float4 z = make_float4(x.x * g[0], x.y * g[1], x.z * g[2], x.w * g[3]);
+            const float top = warp_larger(larger(larger(larger(fabsf(z.x), z.y), z.z), z.w));
+            if (row < rows) {  // the same for the whole warp
+                const Factor factor(top);
+                if (col < width)
+                    *reinterpret_cast<uint32_t*>(a.codes + row * a.code_stride + col) =
+                        codes4(factor(z.x, fmaf(x.x, g[0], -z.x)), factor(z.y, fmaf(x.y, g[1], -z.y)),
+                               factor(z.z, fmaf(x.z, g[2], -z.z)), factor(z.w, fmaf(x.w, g[3], -z.w)));
+                if (lane == 0) a.scales[row * a.scale_stride + blockIdx.x] = scale_of(top) * f;
             }
         }
     }
-    if constexpr (!COLS) return;
 
-    Factor tile_factor(0.0f);
     if constexpr (TILES) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) all_top = max(all_top, __shfl_xor_sync(0xffffffffu, all_top, d));
-        if (lane == 0) s_top[warp][0] = all_top;
+        const float mine = warp_larger(larger(larger(larger(col_top.x, col_top.y), col_top.z), col_top.w));
+        if (lane == 0) s_top[0][warp] = mine;
         __syncthreads();
+        float top = s_top[0][0];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) all_top = max(all_top, s_top[w][0]);
-        const float top = __uint_as_float(all_top);
-        tile_factor = Factor(top);
+        for (int w = 1; w < 8; ++w) top = larger(top, s_top[0][w]);
+        col_top = make_float4(top, top, top, top);
         if (threadIdx.x == 0) {
             if constexpr (ROWS) a.scales[blockIdx.y * a.scale_stride + blockIdx.x] = scale_of(top);
             a.scales_t[blockIdx.x * a.scale_t_stride + blockIdx.y] = scale_of(top);
         }
     } else {
-        if constexpr (kPart == 2) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) col_top[j] = max(col_top[j], __shfl_xor_sync(0xffffffffu, col_top[j], 16));
-        }
-        if (lane < kLanes) {
-#pragma unroll
-            for (int j = 0; j < N; ++j) s_top[warp][col0 + j] = col_top[j];
-        }
+        *reinterpret_cast<float4*>(&s_top[warp][col0]) = col_top;
         __syncthreads();
-        if (threadIdx.x < 128) {
-            uint32_t most = 0;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) most = max(most, s_top[w][threadIdx.x]);
-            s_top[0][threadIdx.x] = most;  // each thread writes only the column that it alone reads
-            const int64_t col = tile_col + threadIdx.x;
-            if (col < width)
-                a.scales_t[col * a.scale_t_stride + blockIdx.y] =
-                    scale_of(__uint_as_float(most)) * (a.col_factor ? a.col_factor[col] : 1.0f);
+        for (int w = 0; w < 8; ++w) {
+            const float4 other = *reinterpret_cast<const float4*>(&s_top[w][col0]);
+            col_top = make_float4(larger(col_top.x, other.x), larger(col_top.y, other.y), larger(col_top.z, other.z),
+                                  larger(col_top.w, other.w));
         }
-        __syncthreads();
+        if (warp == 0) {
+            const float top[4] = {col_top.x, col_top.y, col_top.z, col_top.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < width)
+                    a.scales_t[(col + j) * a.scale_t_stride + blockIdx.y] =
+                        scale_of(top[j]) * (a.col_factor ? a.col_factor[col + j] : 1.0f);
+        }
     }
 
 #pragma unroll
-    for (int j4 = 0; j4 < N; j4 += 4) {
-        uint32_t piece[4][kMine / 4];
-        Factor column[4] = {Factor(0.0f), Factor(0.0f), Factor(0.0f), Factor(0.0f)};
-        if constexpr (!TILES) {
+    for (int j = 0; j < 4; ++j) {
+        const Factor factor(j == 0 ? col_top.x : j == 1 ? col_top.y : j == 2 ? col_top.z : col_top.w);
+        uint32_t piece[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) column[j] = Factor(__uint_as_float(s_top[0][col0 + j4 + j]));
-        }
-#pragma unroll
-        for (int i4 = 0; i4 < kMine; i4 += 4) {
-            float q[4][4];  // [row][column]
+        for (int i4 = 0; i4 < 4; ++i4) {
+            float q[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float z[N];
-                unpack<T>(raw[i4 + i], z);
-                const int64_t row = tile_row + row0 + i4 + i;
-                const float f = !TILES && a.row_factor && row < rows ? a.row_factor[row] : 1.0f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) q[i][j] = TILES ? tile_factor(z[j4 + j]) : column[j](z[j4 + j] * f);
-                if constexpr (TILES && ROWS) {
-                    if (row < rows && tile_col + col0 < width)
-                        *reinterpret_cast<uint32_t*>(a.codes + row * a.code_stride + tile_col + col0 + j4) =
-                            codes4(q[i][0], q[i][1], q[i][2], q[i][3]);
-                }
+                const float x = to_float(reinterpret_cast<const T*>(&raw[i4 * 4 + i])[j]);
+                const float f = row_factor ? s_factor[row0 + i4 * 4 + i] : 1.0f;
+                const float z = x * f;
+                q[i] = factor(z, fmaf(x, f, -z));
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) piece[j][i4 / 4] = codes4(q[0][j], q[1][j], q[2][j], q[3][j]);
+            piece[i4] = codes4(q[0], q[1], q[2], q[3]);
         }
+        *reinterpret_cast<uint4*>(s_codes + (col0 + j) * 128 + (warp ^ (lane & 7)) * 16) =
+            make_uint4(piece[0], piece[1], piece[2], piece[3]);
+    }
+    if constexpr (TILES && ROWS) {
+        const Factor factor(col_top.x);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int col = col0 + j4 + j;
-#pragma unroll
-            for (int k = 0; k < kMine / 8; ++k) {
-                const int at = (row0 / 8 + k) ^ (col / N & 15);
-                *reinterpret_cast<uint2*>(s_codes + col * 128 + at * 8) =
-                    make_uint2(piece[j][2 * k], piece[j][2 * k + 1]);
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int64_t row = tile_row + row0 + i;
+            const float4 x = unpack4<T>(raw[i]);
+            if (row < rows && col < width)
+                *reinterpret_cast<uint32_t*>(a.codes + row * a.code_stride + col) =
+                    codes4(factor(x.x), factor(x.y), factor(x.z), factor(x.w));
         }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int at = k * 256 + threadIdx.x;
-        const int col = at >> 3, pair = at & 7;
-        const int swap = col / N & 15;
-        uint4 v = *reinterpret_cast<const uint4*>(s_codes + col * 128 + ((pair ^ (swap >> 1)) * 16));
-        if (swap & 1) v = make_uint4(v.z, v.w, v.x, v.y);
-        const int64_t row = tile_row + pair * 16;
-        if (tile_col + col < width && row < rows)  // the pitch covers the 16 bytes
-            *reinterpret_cast<uint4*>(a.codes_t + (tile_col + col) * a.code_t_stride + row) = v;
+        const int c = at >> 3, piece = at & 7;
+        const uint4 v = *reinterpret_cast<const uint4*>(s_codes + c * 128 + (piece ^ (c / 4 & 7)) * 16);
+        const int64_t row = tile_row + piece * 16;
+        if (tile_col + c < width && row < rows)  // the pitch covers the 16 bytes
+            *reinterpret_cast<uint4*>(a.codes_t + (tile_col + c) * a.code_t_stride + row) = v;
     }
 }
 
-template <class T, bool ROWS, bool COLS, bool TILES>
+template <class T, bool ROWS, bool TILES>
 void launch_tiles(const TileArgs<T>& a, cudaStream_t stream) {
     const int64_t cols = blocks_of(a.x.width), rows = blocks_of(a.x.rows);
     if (cols == 0 || rows == 0) return;
@@ -614,7 +682,7 @@ void launch_tiles(const TileArgs<T>& a, cudaStream_t stream) {
         if (b.scales) b.scales += (TILES ? r0 : skip) * a.scale_stride;
         if (b.codes_t) b.codes_t += skip;
         if (b.scales_t) b.scales_t += r0;
-        tile_kernel<T, ROWS, COLS, TILES><<<dim3((unsigned)cols, (unsigned)count), 256, 0, stream>>>(b);
+        tile_kernel<T, ROWS, TILES><<<dim3((unsigned)cols, (unsigned)count), 256, 0, stream>>>(b);
         check(cudaGetLastError(), "quantize launch");
     }
 }
@@ -766,10 +834,10 @@ int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride
                                 row_factor, col_factor,
                                 static_cast<uint8_t*>(codes), code_stride, scales, scale_stride,
                                 static_cast<uint8_t*>(codes_t), code_t_stride, scales_t, scale_t_stride};
-            if (tiles && codes) launch_tiles<T, true, true, true>(a, s);
-            else if (tiles) launch_tiles<T, false, true, true>(a, s);
-            else if (codes) launch_tiles<T, true, true, false>(a, s);
-            else launch_tiles<T, false, true, false>(a, s);
+            if (tiles && codes) launch_tiles<T, true, true>(a, s);
+            else if (tiles) launch_tiles<T, false, true>(a, s);
+            else if (codes) launch_tiles<T, true, false>(a, s);
+            else launch_tiles<T, false, false>(a, s);
         });
     });
 }

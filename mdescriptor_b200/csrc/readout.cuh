@@ -158,6 +158,129 @@ __device__ __forceinline__ void store_unit(T* row, int64_t col, int64_t width, c
     }
 }
 
+// ------------------------------------------------------------ quads
+//
+// Four neighbouring elements a lane: a warp holds one block of 128 of a row.
+
+template <class T>
+struct Quad;  // the word that four elements fill
+template <>
+struct Quad<float> { using Word = uint4; };
+template <>
+struct Quad<__nv_bfloat16> { using Word = uint2; };
+template <>
+struct Quad<__half> { using Word = uint2; };
+
+template <class T>
+__device__ __forceinline__ float4 unpack4(const typename Quad<T>::Word& w) {
+    const T* t = reinterpret_cast<const T*>(&w);
+    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
+}
+
+template <class T>
+__device__ __forceinline__ typename Quad<T>::Word pack4(const float4& f) {
+    typename Quad<T>::Word w;
+    T* t = reinterpret_cast<T*>(&w);
+    t[0] = from_float<T>(f.x), t[1] = from_float<T>(f.y), t[2] = from_float<T>(f.z), t[3] = from_float<T>(f.w);
+    return w;
+}
+
+__device__ __forceinline__ uint2 splice(const uint2& a, const uint2& b, int shift) {
+    const uint32_t w0 = shift < 4 ? a.x : a.y, w1 = shift < 4 ? a.y : b.x, w2 = shift < 4 ? b.x : b.y;
+    const int r = (shift & 3) * 8;
+    return make_uint2(__funnelshift_r(w0, w1, r), __funnelshift_r(w1, w2, r));
+}
+
+// Whether a row's quads can be read and written as words.
+template <class T>
+__device__ __forceinline__ bool quads_aligned(const T* row) {
+    return reinterpret_cast<uintptr_t>(row) % sizeof(typename Quad<T>::Word) == 0;
+}
+
+// Elements col .. col + 3 of a row of any alignment, zero past `width`.
+// [begin, end) is the byte range of the whole matrix: the two aligned words
+// that hold a misaligned quad are only read where both lie inside it.
+template <class T>
+__device__ __forceinline__ typename Quad<T>::Word load_quad(const T* row, int64_t col, int64_t width, uintptr_t begin,
+                                                            uintptr_t end) {
+    using Word = typename Quad<T>::Word;
+    const T* p = row + col;
+    Word w{};
+    if (col + 4 <= width) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+        const int shift = (int)(at % sizeof(Word));
+        if (shift == 0) return __ldg(reinterpret_cast<const Word*>(p));
+        const uintptr_t word = at - shift;
+        if (word >= begin && word + 2 * sizeof(Word) <= end) {
+            const Word* q = reinterpret_cast<const Word*>(word);
+            return splice(__ldg(q), __ldg(q + 1), shift);
+        }
+    }
+    T* t = reinterpret_cast<T*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (col + i < width) t[i] = p[i];
+    return w;
+}
+
+// A misaligned quad whose two aligned words may be read.
+template <class T>
+__device__ __forceinline__ typename Quad<T>::Word load_split(const T* p) {
+    using Word = typename Quad<T>::Word;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const int shift = (int)(at % sizeof(Word));
+    const Word* q = reinterpret_cast<const Word*>(at - shift);
+    return shift == 0 ? __ldg(q) : splice(__ldg(q), __ldg(q + 1), shift);
+}
+
+__device__ __forceinline__ uint2 shuffle_up(const uint2& w) {
+    return make_uint2(__shfl_up_sync(0xffffffffu, w.x, 1), __shfl_up_sync(0xffffffffu, w.y, 1));
+}
+__device__ __forceinline__ uint4 shuffle_up(const uint4& w) {
+    return make_uint4(__shfl_up_sync(0xffffffffu, w.x, 1), __shfl_up_sync(0xffffffffu, w.y, 1),
+                      __shfl_up_sync(0xffffffffu, w.z, 1), __shfl_up_sync(0xffffffffu, w.w, 1));
+}
+
+// One quad per lane of a row of any alignment; all 32 lanes, holding
+// consecutive quads, call it together.  Where the row is not aligned to words,
+// each lane joins its quad's head to its lower neighbour's tail and stores that
+// aligned word; the two ends of the warp's stretch go out element by element.
+template <class T>
+__device__ __forceinline__ void store_quad(T* row, int64_t col, int64_t width, const typename Quad<T>::Word& w) {
+    using Word = typename Quad<T>::Word;
+    T* p = row + col;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(row) % sizeof(Word));  // col is a multiple of four
+    const T* t = reinterpret_cast<const T*>(&w);
+    if (shift == 0) {
+        if (col + 4 <= width) {
+            *reinterpret_cast<Word*>(p) = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < width) p[i] = t[i];
+        }
+        return;
+    }
+    const Word below = shuffle_up(w);
+    const int lane = threadIdx.x & 31;
+    const int head = ((int)sizeof(Word) - shift) / (int)sizeof(T);  // elements of a quad below the next aligned word
+    if (lane > 0 && col + head <= width) {
+        *reinterpret_cast<Word*>(p + head - 4) = splice(below, w, (int)sizeof(Word) - shift);
+    } else {
+        const T* b = reinterpret_cast<const T*>(&below);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < head && col + i < width) p[i] = t[i];
+            if (lane > 0 && i >= head && col - 4 + i < width) p[i - 4] = b[i];
+        }
+    }
+    if (lane == 31) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i >= head && col + i < width) p[i] = t[i];
+    }
+}
+
 // kUnit<T> float32 values of a vector from `col` on; zero past `width`.
 template <int N>
 __device__ __forceinline__ void load_vector(const float* v, int64_t col, int64_t width, float (&f)[N]) {
@@ -179,20 +302,33 @@ __device__ __forceinline__ void load_vector(const float* v, int64_t col, int64_t
 // |x| as an unsigned whose order is the magnitudes' with NaN on top.
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// 448 / top as a sum hi + lo, so that fma(z, hi, z * lo) is the correctly
-// rounded quotient's neighbour to within 2^-40: an entry that lies on a tie
-// between two codes is seen as one.  Zero for a block that is stored as zeros.
+// The larger magnitude; NaN if one is.
+__device__ __forceinline__ float larger(float most, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(most), "f"(fabsf(x)));
+    return r;
+}
+// The largest of the warp's magnitudes.
+__device__ __forceinline__ float warp_larger(float most) {
+    float r;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(most));
+    return r;
+}
+
+// 448 / top as a sum hi + lo, good to about 2^-40, so that fma(z, hi, z * lo) is
+// 448 z / top rounded once: an entry that lies on a tie between two codes is
+// seen as one.  Zero for a block that is stored as zeros.
 struct Factor {
     float hi, lo;
     __device__ __forceinline__ explicit Factor(float top) {
-        if (top < kTiny) {
-            hi = lo = 0.0f;
-            return;
-        }
-        hi = __fdiv_rn(kTop, top);
-        lo = top == INFINITY ? 0.0f : __fdiv_rn(fmaf(-hi, top, kTop), top);
+        hi = __fdividef(kTop, top);  // any close value does: lo holds the rest
+        lo = fmaf(-hi, top, kTop) * (hi * (1.0f / kTop));
+        if (!(top < 0x1p126f)) hi = __fdiv_rn(kTop, top), lo = 0.0f;  // infinite and NaN too
+        if (top < kTiny) hi = lo = 0.0f;
     }
     __device__ __forceinline__ float operator()(float z) const { return fmaf(z, hi, z * lo); }
+    // the same for z + rest, the exact product of two floats
+    __device__ __forceinline__ float operator()(float z, float rest) const { return fmaf(z, hi, fmaf(z, lo, rest * hi)); }
 };
 
 __device__ __forceinline__ float scale_of(float top) { return top < kTiny ? 0.0f : __fdiv_rn(top, kTop); }
