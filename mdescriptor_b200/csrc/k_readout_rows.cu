@@ -4,6 +4,7 @@
 #include "host_errors.cuh"
 #include "readout.cuh"
 #include "readout_host.cuh"
+#include "bulk_copy.cuh"
 
 #include <algorithm>
 
@@ -48,19 +49,20 @@ template <class T, bool CTA_ROW, Rows MODE>
 struct RowPass {
     using Word = typename Quad<T>::Word;
     static constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+    static constexpr int kStep = CTA_ROW ? kRowWarps : 1;  // blocks from one of a warp's to its next
     const RowArgs<T>& a;
     const T* x;
     const T* r;  // null without a residual
     T* sum;      // null where it is not wanted
     uint8_t* codes;
     float* top;
-    int64_t width;
+    int width;
     uintptr_t x_begin, x_end, r_begin, r_end;
     float total;
 
-    // One block from its words.  FULL: all 128 columns exist and rows are aligned to words.
+    // One block from its words.  FULL: all 128 columns exist, rows and factors are aligned to words.
     template <bool FULL>
-    __device__ __forceinline__ void block(int64_t col, const Word& wx, const Word& wr) {
+    __device__ __forceinline__ void block(int col, const Word& wx, const Word& wr) {
         const int lane = threadIdx.x & 31;
         float4 s = unpack4<T>(wx);
         if (r) {
@@ -76,14 +78,20 @@ struct RowPass {
         }
         if constexpr (MODE != Rows::NormWide) {
             float4 z = s, rest = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (a.col_factor) {
-                float w[4];
-                load_vector<4>(a.col_factor, col, width, w);
-                z = make_float4(s.x * w[0], s.y * w[1], s.z * w[2], s.w * w[3]);
-                rest = make_float4(fmaf(s.x, w[0], -z.x), fmaf(s.y, w[1], -z.y), fmaf(s.z, w[2], -z.z),
-                                   fmaf(s.w, w[3], -z.w));
+            if (MODE == Rows::Norm8 || a.col_factor) {
+                float4 w;
+                if constexpr (FULL) {
+                    w = __ldg(reinterpret_cast<const float4*>(a.col_factor + col));
+                } else {
+                    float f[4];
+                    load_vector<4>(a.col_factor, col, width, f);
+                    w = make_float4(f[0], f[1], f[2], f[3]);
+                }
+                z = make_float4(s.x * w.x, s.y * w.y, s.z * w.z, s.w * w.w);
+                rest = make_float4(fmaf(s.x, w.x, -z.x), fmaf(s.y, w.y, -z.y), fmaf(s.z, w.z, -z.z),
+                                   fmaf(s.w, w.w, -z.w));
             }
-            const float most = warp_larger(larger(larger(larger(fabsf(z.x), z.y), z.z), z.w));
+            const float most = warp_larger(larger(larger(z.x, z.y, z.z), z.w));
             const Factor factor(most);
             if (FULL || col < width) {  // the pitch covers a quad's padding
                 if (lane == 0) top[col / kBlock] = most;
@@ -95,39 +103,39 @@ struct RowPass {
 
     // kAhead blocks from `b` on, their words loaded first.
     template <bool ALIGNED>
-    __device__ __forceinline__ void several(int b, int step) {
-        const int lane = threadIdx.x & 31;
+    __device__ __forceinline__ void several(int b) {
+        const int col = b * kBlock + (int)(threadIdx.x & 31) * 4;
         Word wx[kAhead], wr[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int64_t col = (int64_t)(b + i * step) * kBlock + lane * 4;
-            wx[i] = ALIGNED ? __ldg(reinterpret_cast<const Word*>(x + col)) : load_split(x + col);
-            wr[i] = !r ? Word{} : ALIGNED ? __ldg(reinterpret_cast<const Word*>(r + col)) : load_split(r + col);
+            const T* px = x + col + i * kStep * kBlock;
+            const T* pr = r + col + i * kStep * kBlock;
+            wx[i] = ALIGNED ? __ldg(reinterpret_cast<const Word*>(px)) : load_split(px);
+            if (r) wr[i] = ALIGNED ? __ldg(reinterpret_cast<const Word*>(pr)) : load_split(pr);
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            block<ALIGNED>((int64_t)(b + i * step) * kBlock + lane * 4, wx[i], wr[i]);
+        for (int i = 0; i < kAhead; ++i) block<ALIGNED>(col + i * kStep * kBlock, wx[i], wr[i]);
     }
 
     // Whether the aligned words around columns [0, columns) of a row lie inside its matrix.
-    __device__ __forceinline__ bool inside(const T* row, int64_t columns, uintptr_t begin, uintptr_t end) const {
+    __device__ __forceinline__ bool inside(const T* row, int columns, uintptr_t begin, uintptr_t end) const {
         const uintptr_t at = reinterpret_cast<uintptr_t>(row), shift = at % sizeof(Word);
         return shift == 0 || (at - shift >= begin && at - shift + columns * sizeof(T) + sizeof(Word) <= end);
     }
 
     // The warp's blocks: kAhead of them under way at a time.
-    __device__ __forceinline__ void run(int first, int step) {
+    __device__ __forceinline__ void run(int first) {
         const int lane = threadIdx.x & 31;
-        const int full = (int)(width / kBlock);
+        const int full = width / kBlock;
         int b = first;
-        if (quads_aligned(x) && (!r || quads_aligned(r)) && (!sum || quads_aligned(sum))) {
-            for (; b + (kAhead - 1) * step < full; b += kAhead * step) several<true>(b, step);
-        } else if (inside(x, (int64_t)full * kBlock, x_begin, x_end) &&
-                   (!r || inside(r, (int64_t)full * kBlock, r_begin, r_end))) {
-            for (; b + (kAhead - 1) * step < full; b += kAhead * step) several<false>(b, step);
+        if (quads_aligned(x) && (!r || quads_aligned(r)) && (!sum || quads_aligned(sum)) &&
+            reinterpret_cast<uintptr_t>(a.col_factor) % 16 == 0) {
+            for (; b + (kAhead - 1) * kStep < full; b += kAhead * kStep) several<true>(b);
+        } else if (inside(x, full * kBlock, x_begin, x_end) && (!r || inside(r, full * kBlock, r_begin, r_end))) {
+            for (; b + (kAhead - 1) * kStep < full; b += kAhead * kStep) several<false>(b);
         }
-        for (; (int64_t)b * kBlock < width; b += step) {
-            const int64_t col = (int64_t)b * kBlock + lane * 4;
+        for (; b * kBlock < width; b += kStep) {
+            const int col = b * kBlock + lane * 4;
             const Word wx = load_quad(x, col, width, x_begin, x_end);
             const Word wr = r ? load_quad(r, col, width, r_begin, r_end) : Word{};
             block<false>(col, wx, wr);
@@ -136,7 +144,7 @@ struct RowPass {
 };
 
 template <class T, bool CTA_ROW, Rows MODE>
-__global__ __launch_bounds__(kRowWarps * 32) void rows_kernel(const __grid_constant__ RowArgs<T> a) {
+__global__ __launch_bounds__(kRowWarps * 32, 4) void rows_kernel(const __grid_constant__ RowArgs<T> a) {
     extern __shared__ float s_top[];
     __shared__ float s_sum[kRowWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -153,12 +161,12 @@ __global__ __launch_bounds__(kRowWarps * 32) void rows_kernel(const __grid_const
                                    MODE != Rows::Quantize && a.sum ? a.sum + row * a.sum_stride : nullptr,
                                    a.codes + row * a.code_stride,
                                    s_top + (CTA_ROW ? 0 : warp * nblocks),
-                                   width,
+                                   (int)width,
                                    reinterpret_cast<uintptr_t>(a.x.data), span_end(a.x.data, a.x.stride),
                                    reinterpret_cast<uintptr_t>(a.residual), span_end(a.residual, a.residual_stride),
                                    0.0f};
     const int first = CTA_ROW ? warp : 0, step = CTA_ROW ? kRowWarps : 1;
-    pass.run(first, step);
+    pass.run(first);
 
     float row_scale = 1.0f;
     if constexpr (MODE != Rows::Quantize) {
@@ -230,11 +238,13 @@ void launch_rows(const RowArgs<T>& a, int sms, cudaStream_t stream) {
 // c = sum_d dy w s;  ds = rstd w dy - s rstd^3 c / D (+ dsum);  dw = sum_t dy s rstd.
 //
 // A CTA takes rows b, b + grid, ...: each thread owns the same NU units of 16
-// bytes of every row, so the row stays in registers between the sum c and the
-// result (the next row's units already under way), and the weight's gradient
-// adds up in registers over the CTA's rows.  The partial sums of all CTAs go to
-// the workspace and are added in CTA order by a second kernel: the same bits on
-// every run.  Bound by HBM: dy, s, dsum once in, ds once out.
+// bytes of every row.  Its units of the next kDepth - 1 rows are on their way
+// into its own slots of a ring in shared memory (nobody else reads them, so no
+// barrier guards them); a row stays in registers between the sum c and the
+// result, and the weight's gradient adds up in registers over the CTA's rows.
+// The partial sums of all CTAs go to the workspace and are added in CTA order by
+// a second kernel: the same bits on every run.  Bound by HBM: dy, s, dsum once
+// in, ds once out.
 //
 // ALIKE: the matrices' rows sit alike relative to 16 bytes.  With an odd width
 // the rows' alignment repeats every eight rows at most; the grid is a multiple of
@@ -254,30 +264,42 @@ struct NormBackwardArgs {
     float* dots;  // wide rows only: c of each row
 };
 
-// The sum over the CTA's warps; `scratch` holds one float a warp.
-__device__ __forceinline__ float cta_sum(float x, float* scratch) {
+// The sum over the CTA's warps (at most 16); `scratch` holds zeros beyond theirs.
+__device__ __forceinline__ float cta_sum(float x, float (&scratch)[16]) {
     x = warp_sum(x);
-    if (blockDim.x == 32) return x;
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
+    float4 part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part[i] = reinterpret_cast<const float4*>(scratch)[i];
     float total = 0.0f;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) total += scratch[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total += (part[i].x + part[i].y) + (part[i].z + part[i].w);
     return total;
 }
+
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(bulk::smem_u32(to)), "l"(from) : "memory");
+}
+
+__host__ __device__ constexpr int ring_depth(int units) { return units == 1 ? 4 : units == 2 ? 3 : 2; }
 
 template <class T, int NU, bool ALIKE>
 __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(const __grid_constant__ NormBackwardArgs<T> a) {
     constexpr int N = kUnit<T>;
-    constexpr bool kAhead = NU <= 2;  // the next row's units are loaded a row ahead; the weight stays in registers
-    __shared__ float scratch[2][16];
+    constexpr int kDepth = ring_depth(NU);
+    constexpr bool kHeld = NU <= 2;  // the weight stays in registers
+    extern __shared__ uint4 ring[];  // [kDepth][3][NU][threads]
+    __shared__ __align__(16) float scratch[2][16];
     const int width = (int)a.s.width, threads = blockDim.x;
     const MatrixIn<T> dsum{a.dsum, a.s.rows, a.s.width, a.dsum_stride};
     const int64_t first = blockIdx.x;
     const int before = ALIKE ? (int)(reinterpret_cast<uintptr_t>(a.s.data + first * a.s.stride) % 16 / sizeof(T)) : 0;
+    if (threadIdx.x < 32) scratch[threadIdx.x / 16][threadIdx.x % 16] = 0.0f;
 
     int col[NU];
     bool whole[NU];
-    float w[kAhead ? NU : 1][N], dw[NU][N];
+    float w[kHeld ? NU : 1][N], dw[NU][N];
     const auto weight_of = [&](int u, float (&f)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) f[i] = col[u] + i >= 0 && col[u] + i < width ? __ldg(a.weight + col[u] + i) : 0.0f;
@@ -286,68 +308,89 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
     for (int u = 0; u < NU; ++u) {
         col[u] = (u * threads + threadIdx.x) * N - before;
         whole[u] = col[u] >= 0 && col[u] + N <= width;
-        if constexpr (kAhead) weight_of(u, w[u]);
+        if constexpr (kHeld) weight_of(u, w[u]);
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[u][i] = 0.0f;
     }
-    const auto load = [&](const MatrixIn<T>& m, int64_t row, int u) {
-        if constexpr (!ALIKE) return m.unit(row, col[u]);
-        const T* p = m.data + row * m.stride + col[u];
-        if (whole[u]) return __ldg(reinterpret_cast<const uint4*>(p));
-        uint4 q = make_uint4(0, 0, 0, 0);
-        T* t = reinterpret_cast<T*>(&q);
+    const auto slot = [&](int stage, int which, int u) -> uint4& {
+        return ring[((stage * 3 + which) * NU + u) * threads + threadIdx.x];
+    };
+    // One unit of a row into its slot.
+    const auto fetch = [&](const MatrixIn<T>& m, int64_t row, int u, uint4& to) {
+        if constexpr (ALIKE) {
+            if (col[u] >= width || col[u] + N <= 0) return;
+            const T* p = m.data + row * m.stride + col[u];
+            if (whole[u] || (p >= m.data && p + N <= m.data + (m.rows - 1) * m.stride + width)) {
+                copy16(&to, p);
+                return;
+            }
+            uint4 q = make_uint4(0, 0, 0, 0);
+            T* t = reinterpret_cast<T*>(&q);
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (col[u] + i >= 0 && col[u] + i < width) t[i] = p[i];
-        return q;
+            for (int i = 0; i < N; ++i)
+                if (col[u] + i >= 0 && col[u] + i < width) t[i] = p[i];
+            to = q;
+        } else {
+            to = m.unit(row, col[u]);
+        }
+    };
+    const auto fetch_row = [&](int64_t row, int stage) {
+        if (row < a.s.rows) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                fetch(a.dy, row, u, slot(stage, 0, u));
+                fetch(a.s, row, u, slot(stage, 1, u));
+                if (a.dsum) fetch(dsum, row, u, slot(stage, 2, u));
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // A unit's floats; zero outside the row.
+    const auto take = [&](const uint4& q, int u, float (&f)[N]) {
+        unpack<T>(q, f);
+        if (!whole[u]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (col[u] + i < 0 || col[u] + i >= width) f[i] = 0.0f;
+        }
     };
 
     const float inv_width = __fdiv_rn(1.0f, (float)width);
-    uint4 qdy[NU], qs[NU], qd[NU], next_dy[NU], next_s[NU], next_d[NU];
-    float rstd = 0.0f, next_rstd = 0.0f;
-    const auto fetch = [&](int64_t row) {
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            next_dy[u] = load(a.dy, row, u);
-            next_s[u] = load(a.s, row, u);
-            if (a.dsum) next_d[u] = load(dsum, row, u);
-        }
-        next_rstd = a.rstd[row];
-    };
-    if (kAhead && first < a.s.rows) fetch(first);
-    int turn = 0;
+    for (int i = 0; i < kDepth - 1; ++i) fetch_row(first + i * (int64_t)gridDim.x, i);
+    float next_rstd = first < a.s.rows ? a.rstd[first] : 0.0f;
+    __syncthreads();  // the zeros of `scratch`
+    int turn = 0, stage = 0;
     for (int64_t row = first; row < a.s.rows; row += gridDim.x, turn ^= 1) {
-        if (!kAhead) fetch(row);
-#pragma unroll
-        for (int u = 0; u < NU; ++u) qdy[u] = next_dy[u], qs[u] = next_s[u], qd[u] = next_d[u];
-        rstd = next_rstd;
-        if (kAhead && row + gridDim.x < a.s.rows) fetch(row + gridDim.x);
+        fetch_row(row + (kDepth - 1) * (int64_t)gridDim.x, stage == 0 ? kDepth - 1 : stage - 1);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        const float rstd = next_rstd;
+        if (row + gridDim.x < a.s.rows) next_rstd = a.rstd[row + gridDim.x];
+        float dy[NU][N], s[NU][N];
         float c = 0.0f;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            float dy[N], s[N], g[N];
-            unpack<T>(qdy[u], dy);
-            unpack<T>(qs[u], s);
-            if constexpr (!kAhead) weight_of(u, g);
+            float g[N];
+            take(slot(stage, 0, u), u, dy[u]);
+            take(slot(stage, 1, u), u, s[u]);
+            if constexpr (!kHeld) weight_of(u, g);
 #pragma unroll
-            for (int i = 0; i < N; ++i) c = fmaf(dy[i] * (kAhead ? w[kAhead ? u : 0][i] : g[i]), s[i], c);
+            for (int i = 0; i < N; ++i) {
+                dw[u][i] = fmaf(dy[u][i], s[u][i] * rstd, dw[u][i]);
+                dy[u][i] *= kHeld ? w[kHeld ? u : 0][i] : g[i];
+                c = fmaf(dy[u][i], s[u][i], c);
+            }
         }
         // two scratch rows in turn: a warp may be one row ahead of another, never two
         c = cta_sum(c, scratch[turn]) * inv_width * rstd * rstd;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            float dy[N], s[N], out[N], g[N];
-            unpack<T>(qdy[u], dy);
-            unpack<T>(qs[u], s);
-            if constexpr (!kAhead) weight_of(u, g);
+            float out[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                dw[u][i] = fmaf(dy[i], s[i] * rstd, dw[u][i]);
-                out[i] = rstd * fmaf(-s[i], c, dy[i] * (kAhead ? w[kAhead ? u : 0][i] : g[i]));
-            }
+            for (int i = 0; i < N; ++i) out[i] = rstd * fmaf(-s[u][i], c, dy[u][i]);
             if (a.dsum) {
                 float d[N];
-                unpack<T>(qd[u], d);
+                unpack<T>(slot(stage, 2, u), d);
 #pragma unroll
                 for (int i = 0; i < N; ++i) out[i] += d[i];
             }
@@ -366,6 +409,7 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
                 store_unit(a.dx + row * a.dx_stride, col[u], width, pack<T>(out));
             }
         }
+        if (++stage == kDepth) stage = 0;
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -378,7 +422,9 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
 template <class T>
 __global__ __launch_bounds__(256) void norm_dots_kernel(const __grid_constant__ NormBackwardArgs<T> a) {
     constexpr int N = kUnit<T>;
-    __shared__ float scratch[8];
+    __shared__ __align__(16) float scratch[16];
+    if (threadIdx.x < 16) scratch[threadIdx.x] = 0.0f;
+    __syncthreads();
     const int64_t row = blockIdx.x;
     float c = 0.0f;
     for (int64_t col = (int64_t)threadIdx.x * N; col < a.s.width; col += 256 * N) {
@@ -496,7 +542,9 @@ void norm_backward(NormBackwardArgs<T> a, float* dweight, const BackwardShape& s
         const auto kernel = s.units == 1   ? (same ? norm_backward_kernel<T, 1, true> : norm_backward_kernel<T, 1, false>)
                             : s.units == 2 ? (same ? norm_backward_kernel<T, 2, true> : norm_backward_kernel<T, 2, false>)
                                            : (same ? norm_backward_kernel<T, 4, true> : norm_backward_kernel<T, 4, false>);
-        kernel<<<(unsigned)s.grid, s.threads, 0, stream>>>(a);
+        const int bytes = ring_depth(s.units) * 3 * s.units * s.threads * 16;  // at most 192 KB
+        check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "norm gradient ring");
+        kernel<<<(unsigned)s.grid, s.threads, bytes, stream>>>(a);
     } else {
         a.dots = a.partial + s.grid * s.pitch;
         norm_dots_kernel<T><<<(unsigned)a.s.rows, 256, 0, stream>>>(a);
@@ -542,7 +590,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
     using Word = typename Quad<T>::Word;
     __shared__ __align__(16) uint8_t s_codes[128 * 128];
     __shared__ __align__(16) float s_top[8][128];
-    __shared__ float s_factor[128];
+    __shared__ __align__(16) float s_factor[128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t tile_row = (int64_t)blockIdx.y * 128, tile_col = (int64_t)blockIdx.x * 128;
     const int row0 = warp * 16, col0 = lane * 4;
@@ -573,23 +621,46 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
 
     float4 col_top = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float4 x = unpack4<T>(raw[i]);
-        const int64_t row = tile_row + row0 + i;
-        const float f = row_factor ? s_factor[row0 + i] : 1.0f;
-        col_top = make_float4(larger(col_top.x, x.x * f), larger(col_top.y, x.y * f), larger(col_top.z, x.z * f),
-                              larger(col_top.w, x.w * f));
-        if constexpr (ROWS && !TILES) {
-            const float4 z = make_float4(x.x * g[0], x.y * g[1], x.z * g[2], x.w * g[3]);
-            const float top = warp_larger(larger(larger(larger(fabsf(z.x), z.y), z.z), z.w));
-            if (row < rows) {  // the same for the whole warp
-                const Factor factor(top);
-                if (col < width)
-                    *reinterpret_cast<uint32_t*>(a.codes + row * a.code_stride + col) =
-                        codes4(factor(z.x, fmaf(x.x, g[0], -z.x)), factor(z.y, fmaf(x.y, g[1], -z.y)),
-                               factor(z.z, fmaf(x.z, g[2], -z.z)), factor(z.w, fmaf(x.w, g[3], -z.w)));
-                if (lane == 0) a.scales[row * a.scale_stride + blockIdx.x] = scale_of(top) * f;
+    for (int i = 0; i < 16; i += 2) {
+        float4 x = unpack4<T>(raw[i]), y = unpack4<T>(raw[i + 1]);
+        if (row_factor) {
+            const float2 f = *reinterpret_cast<const float2*>(&s_factor[row0 + i]);
+            x.x *= f.x, x.y *= f.x, x.z *= f.x, x.w *= f.x;
+            y.x *= f.y, y.y *= f.y, y.z *= f.y, y.w *= f.y;
+        }
+        col_top = make_float4(larger(col_top.x, x.x, y.x), larger(col_top.y, x.y, y.y), larger(col_top.z, x.z, y.z),
+                              larger(col_top.w, x.w, y.w));
+    }
+    if constexpr (ROWS && !TILES) {
+        // The rows' maxima first; lane i then works out row i's factor for all lanes.
+        float mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float4 x = unpack4<T>(raw[i]);
+            if (col_factor) x.x *= g[0], x.y *= g[1], x.z *= g[2], x.w *= g[3];
+            const float top = warp_larger(larger(larger(x.x, x.y, x.z), x.w));
+            if (lane == i) mine = top;
+        }
+        const Factor own(mine);
+        const int64_t own_row = tile_row + row0 + lane;
+        if (lane < 16 && own_row < rows)
+            a.scales[own_row * a.scale_stride + blockIdx.x] = scale_of(mine) * (row_factor ? s_factor[row0 + lane] : 1.0f);
+        uint8_t* out = a.codes + (tile_row + row0) * a.code_stride + col;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float4 x = unpack4<T>(raw[i]);
+            Factor factor(0.0f);
+            factor.hi = __shfl_sync(0xffffffffu, own.hi, i);
+            factor.lo = __shfl_sync(0xffffffffu, own.lo, i);
+            uint32_t q;
+            if (col_factor) {
+                const float4 z = make_float4(x.x * g[0], x.y * g[1], x.z * g[2], x.w * g[3]);
+                q = codes4(factor(z.x, fmaf(x.x, g[0], -z.x)), factor(z.y, fmaf(x.y, g[1], -z.y)),
+                           factor(z.z, fmaf(x.z, g[2], -z.z)), factor(z.w, fmaf(x.w, g[3], -z.w)));
+            } else {
+                q = codes4(factor(x.x), factor(x.y), factor(x.z), factor(x.w));
             }
+            if (tile_row + row0 + i < rows && col < width) *reinterpret_cast<uint32_t*>(out + i * a.code_stride) = q;
         }
     }
 
@@ -627,18 +698,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const Factor factor(j == 0 ? col_top.x : j == 1 ? col_top.y : j == 2 ? col_top.z : col_top.w);
+        const auto entry = [&](int i) { return to_float(reinterpret_cast<const T*>(&raw[i])[j]); };
         uint32_t piece[4];
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-            float q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = to_float(reinterpret_cast<const T*>(&raw[i4 * 4 + i])[j]);
-                const float f = row_factor ? s_factor[row0 + i4 * 4 + i] : 1.0f;
-                const float z = x * f;
-                q[i] = factor(z, fmaf(x, f, -z));
+        for (int i = 0; i < 16; i += 4) {
+            if (row_factor) {
+                const float4 f = *reinterpret_cast<const float4*>(&s_factor[row0 + i]);
+                const float4 z = make_float4(entry(i) * f.x, entry(i + 1) * f.y, entry(i + 2) * f.z, entry(i + 3) * f.w);
+                piece[i / 4] = codes4(factor(z.x, fmaf(entry(i), f.x, -z.x)), factor(z.y, fmaf(entry(i + 1), f.y, -z.y)),
+                                      factor(z.z, fmaf(entry(i + 2), f.z, -z.z)), factor(z.w, fmaf(entry(i + 3), f.w, -z.w)));
+            } else {
+                piece[i / 4] = codes4(factor(entry(i)), factor(entry(i + 1)), factor(entry(i + 2)), factor(entry(i + 3)));
             }
-            piece[i4] = codes4(q[0], q[1], q[2], q[3]);
         }
         *reinterpret_cast<uint4*>(s_codes + (col0 + j) * 128 + (warp ^ (lane & 7)) * 16) =
             make_uint4(piece[0], piece[1], piece[2], piece[3]);

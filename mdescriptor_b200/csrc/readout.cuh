@@ -308,6 +308,11 @@ __device__ __forceinline__ float larger(float most, float x) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(most), "f"(fabsf(x)));
     return r;
 }
+__device__ __forceinline__ float larger(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 // The largest of the warp's magnitudes.
 __device__ __forceinline__ float warp_larger(float most) {
     float r;
@@ -321,9 +326,10 @@ __device__ __forceinline__ float warp_larger(float most) {
 struct Factor {
     float hi, lo;
     __device__ __forceinline__ explicit Factor(float top) {
-        hi = __fdividef(kTop, top);  // any close value does: lo holds the rest
+        // any close value does for hi, lo holds the rest; 2^-10 keeps the quick division's divisor below 2^126
+        hi = __fdividef(kTop * 0x1p-10f, top * 0x1p-10f);
         lo = fmaf(-hi, top, kTop) * (hi * (1.0f / kTop));
-        if (!(top < 0x1p126f)) hi = __fdiv_rn(kTop, top), lo = 0.0f;  // infinite and NaN too
+        if (top == INFINITY) lo = 0.0f;
         if (top < kTiny) hi = lo = 0.0f;
     }
     __device__ __forceinline__ float operator()(float z) const { return fmaf(z, hi, z * lo); }
