@@ -299,6 +299,7 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
 
     int col[NU];
     bool whole[NU];
+    uint4 mask[NU];  // the bits of a unit that lie inside the row
     float w[kHeld ? NU : 1][N], dw[NU][N];
     const auto weight_of = [&](int u, float (&f)[N]) {
 #pragma unroll
@@ -308,6 +309,12 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
     for (int u = 0; u < NU; ++u) {
         col[u] = (u * threads + threadIdx.x) * N - before;
         whole[u] = col[u] >= 0 && col[u] + N <= width;
+        uint32_t bits[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (col[u] + i >= 0 && col[u] + i < width)
+                bits[i * 4 / N] |= (sizeof(T) == 4 ? 0xffffffffu : 0xffffu) << (sizeof(T) == 4 ? 0 : i % 2 * 16);
+        mask[u] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
         if constexpr (kHeld) weight_of(u, w[u]);
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[u][i] = 0.0f;
@@ -315,54 +322,58 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
     const auto slot = [&](int stage, int which, int u) -> uint4& {
         return ring[((stage * 3 + which) * NU + u) * threads + threadIdx.x];
     };
-    // One unit of a row into its slot.
-    const auto fetch = [&](const MatrixIn<T>& m, int64_t row, int u, uint4& to) {
+    // One unit of a row into its slot; `p` is the unit's address.
+    const auto fetch = [&](const MatrixIn<T>& m, const T* p, int64_t row, int u, uint4& to) {
         if constexpr (ALIKE) {
-            if (col[u] >= width || col[u] + N <= 0) return;
-            const T* p = m.data + row * m.stride + col[u];
-            if (whole[u] || (p >= m.data && p + N <= m.data + (m.rows - 1) * m.stride + width)) {
+            if (whole[u]) {
                 copy16(&to, p);
-                return;
-            }
-            uint4 q = make_uint4(0, 0, 0, 0);
-            T* t = reinterpret_cast<T*>(&q);
+            } else if (col[u] < width && col[u] + N > 0) {
+                if (p >= m.data && p + N <= m.data + (m.rows - 1) * m.stride + width) {
+                    copy16(&to, p);
+                    return;
+                }
+                uint4 q = make_uint4(0, 0, 0, 0);
+                T* t = reinterpret_cast<T*>(&q);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (col[u] + i >= 0 && col[u] + i < width) t[i] = p[i];
-            to = q;
+                for (int i = 0; i < N; ++i)
+                    if (col[u] + i >= 0 && col[u] + i < width) t[i] = p[i];
+                to = q;
+            }
         } else {
             to = m.unit(row, col[u]);
         }
     };
-    const auto fetch_row = [&](int64_t row, int stage) {
-        if (row < a.s.rows) {
+    // The row that is fetched next, and its addresses.
+    int64_t ahead = first;
+    const T *next_dy = a.dy.data + first * a.dy.stride, *next_s = a.s.data + first * a.s.stride,
+            *next_d = a.dsum ? a.dsum + first * a.dsum_stride : nullptr;
+    const int64_t step_dy = a.dy.stride * gridDim.x, step_s = a.s.stride * gridDim.x, step_d = a.dsum_stride * gridDim.x;
+    const auto fetch_row = [&](int stage) {
+        if (ahead < a.s.rows) {
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                fetch(a.dy, row, u, slot(stage, 0, u));
-                fetch(a.s, row, u, slot(stage, 1, u));
-                if (a.dsum) fetch(dsum, row, u, slot(stage, 2, u));
+                fetch(a.dy, next_dy + col[u], ahead, u, slot(stage, 0, u));
+                fetch(a.s, next_s + col[u], ahead, u, slot(stage, 1, u));
+                if (a.dsum) fetch(dsum, next_d + col[u], ahead, u, slot(stage, 2, u));
             }
         }
+        ahead += gridDim.x, next_dy += step_dy, next_s += step_s, next_d += step_d;
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // A unit's floats; zero outside the row.
     const auto take = [&](const uint4& q, int u, float (&f)[N]) {
-        unpack<T>(q, f);
-        if (!whole[u]) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (col[u] + i < 0 || col[u] + i >= width) f[i] = 0.0f;
-        }
+        unpack<T>(make_uint4(q.x & mask[u].x, q.y & mask[u].y, q.z & mask[u].z, q.w & mask[u].w), f);
     };
 
     const float inv_width = __fdiv_rn(1.0f, (float)width);
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) fetch_row(first + i * (int64_t)gridDim.x, i);
+    for (int i = 0; i < kDepth - 1; ++i) fetch_row(i);
     float next_rstd = first < a.s.rows ? a.rstd[first] : 0.0f;
     __syncthreads();  // the zeros of `scratch`
     int turn = 0, stage = 0;
-    for (int64_t row = first; row < a.s.rows; row += gridDim.x, turn ^= 1) {
-        fetch_row(row + (kDepth - 1) * (int64_t)gridDim.x, stage == 0 ? kDepth - 1 : stage - 1);
+    T* dx = a.dx + first * a.dx_stride;
+    for (int64_t row = first; row < a.s.rows; row += gridDim.x, dx += a.dx_stride * gridDim.x, turn ^= 1) {
+        fetch_row(stage == 0 ? kDepth - 1 : stage - 1);
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
         const float rstd = next_rstd;
         if (row + gridDim.x < a.s.rows) next_rstd = a.rstd[row + gridDim.x];
@@ -382,31 +393,30 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
             }
         }
         // two scratch rows in turn: a warp may be one row ahead of another, never two
-        c = cta_sum(c, scratch[turn]) * inv_width * rstd * rstd;
+        c = cta_sum(c, scratch[turn]) * inv_width * rstd * rstd * rstd;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             float out[N];
-#pragma unroll
-            for (int i = 0; i < N; ++i) out[i] = rstd * fmaf(-s[u][i], c, dy[u][i]);
             if (a.dsum) {
-                float d[N];
-                unpack<T>(slot(stage, 2, u), d);
+                unpack<T>(slot(stage, 2, u), out);
+            } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i) out[i] += d[i];
+                for (int i = 0; i < N; ++i) out[i] = 0.0f;
             }
+#pragma unroll
+            for (int i = 0; i < N; ++i) out[i] = fmaf(-s[u][i], c, fmaf(dy[u][i], rstd, out[i]));
             if constexpr (ALIKE) {
-                T* p = a.dx + row * a.dx_stride + col[u];
                 const uint4 q = pack<T>(out);
                 if (whole[u]) {
-                    *reinterpret_cast<uint4*>(p) = q;
-                } else {
+                    *reinterpret_cast<uint4*>(dx + col[u]) = q;
+                } else if (col[u] < width && col[u] + N > 0) {
                     const T* t = reinterpret_cast<const T*>(&q);
 #pragma unroll
                     for (int i = 0; i < N; ++i)
-                        if (col[u] + i >= 0 && col[u] + i < width) p[i] = t[i];
+                        if (col[u] + i >= 0 && col[u] + i < width) dx[col[u] + i] = t[i];
                 }
             } else {
-                store_unit(a.dx + row * a.dx_stride, col[u], width, pack<T>(out));
+                store_unit(dx, col[u], width, pack<T>(out));
             }
         }
         if (++stage == kDepth) stage = 0;
@@ -703,10 +713,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             if (row_factor) {
-                const float4 f = *reinterpret_cast<const float4*>(&s_factor[row0 + i]);
-                const float4 z = make_float4(entry(i) * f.x, entry(i + 1) * f.y, entry(i + 2) * f.z, entry(i + 3) * f.w);
-                piece[i / 4] = codes4(factor(z.x, fmaf(entry(i), f.x, -z.x)), factor(z.y, fmaf(entry(i + 1), f.y, -z.y)),
-                                      factor(z.z, fmaf(entry(i + 2), f.z, -z.z)), factor(z.w, fmaf(entry(i + 3), f.w, -z.w)));
+                const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(&s_factor[row0 + i]);
+                float q[4];
+                factor.pair(entry(i), entry(i + 1), f.x, q[0], q[1]);
+                factor.pair(entry(i + 2), entry(i + 3), f.y, q[2], q[3]);
+                piece[i / 4] = codes4(q[0], q[1], q[2], q[3]);
             } else {
                 piece[i / 4] = codes4(factor(entry(i)), factor(entry(i + 1)), factor(entry(i + 2)), factor(entry(i + 3)));
             }

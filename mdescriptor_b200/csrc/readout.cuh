@@ -333,6 +333,21 @@ struct Factor {
         if (top < kTiny) hi = lo = 0.0f;
     }
     __device__ __forceinline__ float operator()(float z) const { return fmaf(z, hi, z * lo); }
+    // the same for two exact products x f, in packed arithmetic
+    __device__ __forceinline__ void pair(float x, float y, uint64_t f, float& q, float& r) const {
+        asm("{\n\t.reg .b64 x, z, n, e, h, l, q;\n\t"
+            "mov.b64 x, {%2, %3};\n\tmov.b64 h, {%5, %5};\n\tmov.b64 l, {%6, %6};\n\t"
+            "mov.b64 n, {%7, %7};\n\t"
+            "mul.rn.f32x2 z, x, %4;\n\t"
+            "mul.rn.f32x2 n, z, n;\n\t"
+            "fma.rn.f32x2 e, x, %4, n;\n\t"
+            "mul.rn.f32x2 e, e, h;\n\t"
+            "fma.rn.f32x2 e, z, l, e;\n\t"
+            "fma.rn.f32x2 q, z, h, e;\n\t"
+            "mov.b64 {%0, %1}, q;\n\t}"
+            : "=f"(q), "=f"(r)
+            : "f"(x), "f"(y), "l"(f), "f"(hi), "f"(lo), "f"(-1.0f));
+    }
     // the same for z + rest, the exact product of two floats
     __device__ __forceinline__ float operator()(float z, float rest) const { return fmaf(z, hi, fmaf(z, lo, rest * hi)); }
 };
