@@ -56,14 +56,6 @@ __device__ __forceinline__ uint32_t noise(int64_t element, uint32_t key) {
     return h ^ h >> 16;
 }
 
-// a >= 0 (at most 448) down to an e4m3 value after adding u / 2^16 of that
-// value's step.  Above 2^-6 the step is bit 20 of the float; below it is 2^-9.
-__device__ __forceinline__ float dither(float a, uint32_t u) {
-    const float normal = __uint_as_float((__float_as_uint(a) + (u << 4)) & 0xfff00000u);
-    const float low = floorf(fmaf((float)u, 0x1p-16f, a * 512.0f)) * 0x1p-9f;
-    return fminf(a >= 0x1p-6f ? normal : low, kTop);
-}
-
 template <class T>
 __device__ __forceinline__ void load4(const T* p, int64_t at, int64_t count, bool vector, float (&f)[4]) {
     if (vector && at + 4 <= count) {
@@ -101,51 +93,79 @@ __device__ __forceinline__ void store4(T* p, int64_t at, int64_t count, bool vec
         if (at + i < count) p[at + i] = from_float<T>(f[i]);
 }
 
-__device__ __forceinline__ void load_codes4(const uint8_t* p, int64_t at, int64_t count, bool vector, float scale,
-                                            float (&f)[4]) {
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t at, int64_t count, bool vector) {
+    if (vector && at + 4 <= count) return *reinterpret_cast<const uint32_t*>(p + at);
     uint32_t q = 0;
-    if (vector && at + 4 <= count) {
-        q = *reinterpret_cast<const uint32_t*>(p + at);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at + i < count) q |= (uint32_t)p[at + i] << (8 * i);
+    for (int i = 0; i < 4; ++i)
+        if (at + i < count) q |= (uint32_t)p[at + i] << (8 * i);
+    return q;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* p, int64_t at, int64_t count, bool vector, uint32_t codes) {
+    if (vector && at + 4 <= count) {
+        *reinterpret_cast<uint32_t*>(p + at) = codes;
+        return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        __nv_fp8_e4m3 c;
-        c.__x = (uint8_t)(q >> (8 * i));
-        f[i] = (float)c * scale;
+    for (int i = 0; i < 4; ++i)
+        if (at + i < count) p[at + i] = (uint8_t)(codes >> (8 * i));
+}
+
+__device__ __forceinline__ void decode(uint32_t codes, float scale, float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (16 * i)), __NV_E4M3);
+        const float2 t = __half22float2(__half2(h));
+        f[2 * i] = t.x * scale, f[2 * i + 1] = t.y * scale;
     }
 }
 
-// New codes and scale of the warp's block of 128 values (four a lane).
-__device__ __forceinline__ void store_codes4(uint8_t* p, float* scales, int64_t at, int64_t count, bool vector,
-                                             const float (&x)[4], const uint32_t (&u)[4], bool positive) {
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) most = max(most, magnitude(x[i]));
-    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, most));
-    const float scale = top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop);
-    float q[4];
+// Codes of four values of the warp's block of 128, and the block's scale.
+// a = |x| / scale (at most 448) goes down to an e4m3 value after u / 2^16 of
+// that value's step has been added; `u20` holds the u, times 16.  From 2^-6 on
+// the step is bit 20 of the float, so the sum's top bits are the code; below it
+// is 2^-9 (rare: the warp looks whether it has such values at all).  The
+// quotient is x times the rounded reciprocal with one correction (Markstein's
+// method).  FLOOR: a positive x keeps at least the smallest code.
+template <bool FLOOR>
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&u20)[4], float& scale) {
+    const float top = warp_larger(larger(larger(x[0], x[1], x[2]), x[3]));
+    scale = top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop);
+    const float inverse = __frcp_rn(scale);
+    float a[4], least = kTop;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float a = __fdiv_rn(fabsf(x[i]), scale);
-        float c = dither(a, u[i]);
-        if (positive && c == 0.0f && x[i] > 0.0f) c = 0x1p-9f;
-        if (scale == 0.0f) c = 0.0f;
-        if (!(a == a) && scale != 0.0f) c = a;  // NaN stays
-        q[i] = copysignf(c, x[i]);
+        const float q = fabsf(x[i]) * inverse;
+        a[i] = fmaf(fmaf(-q, scale, fabsf(x[i])), inverse, q);
+        least = fminf(least, a[i]);
     }
-    const uint32_t codes = codes4(q[0], q[1], q[2], q[3]);
-    if (vector && at + 4 <= count) {
-        *reinterpret_cast<uint32_t*>(p + at) = codes;
-    } else {
+    uint32_t code[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at + i < count) p[at + i] = (uint8_t)(codes >> (8 * i));
+    for (int i = 0; i < 4; ++i) code[i] = (__float_as_uint(a[i]) + u20[i] - (960u << 20)) >> 20;
+    if (__any_sync(0xffffffffu, least < 0x1p-6f)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float u = __uint_as_float(0x3f800000u | u20[i] << 3) - 1.0f;
+            const float t = __fadd_rd(fmaf(a[i], 512.0f, u), 0x1p23f);  // floor into the low bits
+            if (a[i] < 0x1p-6f) code[i] = __float_as_uint(t) & 15u;
+            if (FLOOR && code[i] == 0 && x[i] > 0.0f) code[i] = 1;
+        }
     }
-    if ((threadIdx.x & 31) == 0 && at < count) scales[at / kBlock] = scale;
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t c = min(code[i], 0x7eu);
+        if (!FLOOR) c |= __float_as_uint(x[i]) >> 24 & 0x80u;
+        codes |= c << (8 * i);
+    }
+    return scale == 0.0f ? 0u : codes;
+}
+
+__device__ __forceinline__ float square_root(float x) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // One CTA a tile of 4096 elements of one tensor.
@@ -158,52 +178,95 @@ __device__ __forceinline__ void store_codes4(uint8_t* p, float* scales, int64_t 
 // lie 1/16 to 1/8 apart, so to the nearest code v would stay where it is.  v
 // itself is stored and not its root, whose dithering noise squared would add
 // to v more than b2 takes away; a positive v keeps at least the smallest code,
-// since a zero under a non-zero m would make a huge step.
+// since a zero under a non-zero m would make a huge step.  A NaN or infinite
+// moment shows in its block's scale.
 // Bound by HBM: p, m, v in and out, g in.
 template <class P, class G, bool SMALL>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const __grid_constant__ StepArgs a) {
-    const Tile tile = a.tiles[blockIdx.x];
-    const Tensor t = a.tensors[tile.tensor];
-    const G* g = static_cast<const G*>(a.grads[tile.tensor - a.first_tensor]);
-    P* p = static_cast<P*>(t.p);
-    const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
-    const float keep = 1.0f - a.lr * t.decay;
-#pragma unroll
-    for (int k = 0; k < kTileUnits; ++k) {
-        const int64_t at = tile.start + (k * kThreads + threadIdx.x) * kSpan;
-        if (tile.start + (k * kThreads + (threadIdx.x & ~31)) * kSpan >= t.count) break;  // the whole warp
+struct Update {
+    const StepArgs& a;
+    const Tensor& t;
+    const G* g;
+    float keep;
+
+    struct Unit {
         float x[4], y[4], m[4], v[4];
-        load4(p, at, t.count, vec_p, x);
-        load4(g, at, t.count, vec_g, y);
+        uint32_t qm, qv;
+        float sm, sv;
+    };
+
+    __device__ __forceinline__ void load(Unit& u, int64_t at, bool vec_p, bool vec_g) const {
+        load4(static_cast<const P*>(t.p), at, t.count, vec_p, u.x);
+        load4(g, at, t.count, vec_g, u.y);
         if constexpr (SMALL) {
-            const int64_t block = min(at, t.count - 1) / kBlock;
-            load_codes4(static_cast<const uint8_t*>(t.m), at, t.count, vec_p, t.m_scale[block], m);
-            load_codes4(static_cast<const uint8_t*>(t.v), at, t.count, vec_p, t.v_scale[block], v);
+            const int64_t block = at / kBlock;  // of the warp's first lane's element: at least that one exists
+            u.qm = load_codes(static_cast<const uint8_t*>(t.m), at, t.count, vec_p);
+            u.qv = load_codes(static_cast<const uint8_t*>(t.v), at, t.count, vec_p);
+            u.sm = t.m_scale[block], u.sv = t.v_scale[block];
         } else {
-            load4(static_cast<const float*>(t.m), at, t.count, vec_p, m);
-            load4(static_cast<const float*>(t.v), at, t.count, vec_p, v);
+            load4(static_cast<const float*>(t.m), at, t.count, vec_p, u.m);
+            load4(static_cast<const float*>(t.v), at, t.count, vec_p, u.v);
+        }
+    }
+
+    __device__ __forceinline__ void finish(Unit& u, int64_t at, bool vec_p) const {
+        if constexpr (SMALL) {
+            decode(u.qm, u.sm, u.m);
+            decode(u.qv, u.sv, u.v);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float grad = y[i] * a.grad_scale;
+            const float grad = u.y[i] * a.grad_scale;
             // products rounded, then the sum: the states' codes depend on every bit of it
-            m[i] = __fadd_rn(__fmul_rn(a.beta1, m[i]), __fmul_rn(a.rest1, grad));
-            v[i] = __fadd_rn(__fmul_rn(a.beta2, v[i]), __fmul_rn(__fmul_rn(a.rest2, grad), grad));
-            x[i] = fmaf(-a.step_size, __fdiv_rn(m[i], fmaf(__fsqrt_rn(v[i]), a.root2, a.eps)), x[i] * keep);
+            u.m[i] = __fadd_rn(__fmul_rn(a.beta1, u.m[i]), __fmul_rn(a.rest1, grad));
+            u.v[i] = __fadd_rn(__fmul_rn(a.beta2, u.v[i]), __fmul_rn(__fmul_rn(a.rest2, grad), grad));
+            const float root = fmaf(square_root(u.v[i]), a.root2, a.eps);
+            u.x[i] = fmaf(-a.step_size, __fdividef(u.m[i], root), u.x[i] * keep);
         }
-        store4(p, at, t.count, vec_p, x);
+        store4(static_cast<P*>(t.p), at, t.count, vec_p, u.x);
         if constexpr (SMALL) {
             uint32_t um[4], uv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t h = noise(t.first + at + i, a.key);
-                um[i] = h >> 16, uv[i] = h & 0xffffu;
+                um[i] = h >> 12 & 0xffff0u, uv[i] = h << 4 & 0xffff0u;
             }
-            store_codes4(static_cast<uint8_t*>(t.m), t.m_scale, at, t.count, vec_p, m, um, false);
-            store_codes4(static_cast<uint8_t*>(t.v), t.v_scale, at, t.count, vec_p, v, uv, true);
+            float sm, sv;
+            store_codes(static_cast<uint8_t*>(t.m), at, t.count, vec_p, encode<false>(u.m, um, sm));
+            store_codes(static_cast<uint8_t*>(t.v), at, t.count, vec_p, encode<true>(u.v, uv, sv));
+            if ((threadIdx.x & 31) == 0) t.m_scale[at / kBlock] = sm, t.v_scale[at / kBlock] = sv;
         } else {
-            store4(static_cast<float*>(t.m), at, t.count, vec_p, m);
-            store4(static_cast<float*>(t.v), at, t.count, vec_p, v);
+            store4(static_cast<float*>(t.m), at, t.count, vec_p, u.m);
+            store4(static_cast<float*>(t.v), at, t.count, vec_p, u.v);
+        }
+    }
+};
+
+template <class P, class G, bool SMALL>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const __grid_constant__ StepArgs a) {
+    const Tile tile = a.tiles[blockIdx.x];
+    const Tensor t = a.tensors[tile.tensor];
+    const G* g = static_cast<const G*>(a.grads[tile.tensor - a.first_tensor]);
+    const Update<P, G, SMALL> update{a, t, g, 1.0f - a.lr * t.decay};
+    const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
+    const int64_t first = tile.start + threadIdx.x * kSpan;
+    if (vec_p && vec_g && tile.start + kTile <= t.count) {
+#pragma unroll
+        for (int k = 0; k < kTileUnits; k += 2) {  // two units under way
+            typename Update<P, G, SMALL>::Unit u[2];
+            const int64_t at = first + k * kThreads * kSpan;
+            update.load(u[0], at, true, true);
+            update.load(u[1], at + kThreads * kSpan, true, true);
+            update.finish(u[0], at, true);
+            update.finish(u[1], at + kThreads * kSpan, true);
+        }
+    } else {
+#pragma unroll 1
+        for (int k = 0; k < kTileUnits; ++k) {
+            const int64_t at = first + k * kThreads * kSpan;
+            if (at - (threadIdx.x & 31) * kSpan >= t.count) break;  // the whole warp
+            typename Update<P, G, SMALL>::Unit u;
+            update.load(u, at, vec_p, vec_g);
+            update.finish(u, at, vec_p);
         }
     }
 }

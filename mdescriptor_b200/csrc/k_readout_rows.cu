@@ -319,9 +319,12 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[u][i] = 0.0f;
     }
-    const auto slot = [&](int stage, int which, int u) -> uint4& {
-        return ring[((stage * 3 + which) * NU + u) * threads + threadIdx.x];
-    };
+    bool all_whole = true;  // of the warp's lanes and units
+#pragma unroll
+    for (int u = 0; u < NU; ++u) all_whole = all_whole && __all_sync(0xffffffffu, whole[u]);
+    // Slots of dy, s and dsum of a stage follow each other, `threads` apart.
+    const int span = 3 * NU * threads;
+    uint4* const mine = ring + threadIdx.x;
     // One unit of a row into its slot; `p` is the unit's address.
     const auto fetch = [&](const MatrixIn<T>& m, const T* p, int64_t row, int u, uint4& to) {
         if constexpr (ALIKE) {
@@ -348,13 +351,22 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
     const T *next_dy = a.dy.data + first * a.dy.stride, *next_s = a.s.data + first * a.s.stride,
             *next_d = a.dsum ? a.dsum + first * a.dsum_stride : nullptr;
     const int64_t step_dy = a.dy.stride * gridDim.x, step_s = a.s.stride * gridDim.x, step_d = a.dsum_stride * gridDim.x;
-    const auto fetch_row = [&](int stage) {
+    const auto fetch_row = [&](uint4* to) {
         if (ahead < a.s.rows) {
+            if (ALIKE && all_whole) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                fetch(a.dy, next_dy + col[u], ahead, u, slot(stage, 0, u));
-                fetch(a.s, next_s + col[u], ahead, u, slot(stage, 1, u));
-                if (a.dsum) fetch(dsum, next_d + col[u], ahead, u, slot(stage, 2, u));
+                for (int u = 0; u < NU; ++u, to += 3 * threads) {
+                    copy16(to, next_dy + col[u]);
+                    copy16(to + threads, next_s + col[u]);
+                    if (a.dsum) copy16(to + 2 * threads, next_d + col[u]);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < NU; ++u, to += 3 * threads) {
+                    fetch(a.dy, next_dy + col[u], ahead, u, to[0]);
+                    fetch(a.s, next_s + col[u], ahead, u, to[threads]);
+                    if (a.dsum) fetch(dsum, next_d + col[u], ahead, u, to[2 * threads]);
+                }
             }
         }
         ahead += gridDim.x, next_dy += step_dy, next_s += step_s, next_d += step_d;
@@ -367,13 +379,14 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
 
     const float inv_width = __fdiv_rn(1.0f, (float)width);
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) fetch_row(i);
+    for (int i = 0; i < kDepth - 1; ++i) fetch_row(mine + i * span);
     float next_rstd = first < a.s.rows ? a.rstd[first] : 0.0f;
     __syncthreads();  // the zeros of `scratch`
-    int turn = 0, stage = 0;
+    int turn = 0;
+    uint4 *now = mine, *behind = mine + (kDepth - 1) * span;  // the slots of this row and of the one before it
     T* dx = a.dx + first * a.dx_stride;
     for (int64_t row = first; row < a.s.rows; row += gridDim.x, dx += a.dx_stride * gridDim.x, turn ^= 1) {
-        fetch_row(stage == 0 ? kDepth - 1 : stage - 1);
+        fetch_row(behind);
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
         const float rstd = next_rstd;
         if (row + gridDim.x < a.s.rows) next_rstd = a.rstd[row + gridDim.x];
@@ -382,8 +395,8 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             float g[N];
-            take(slot(stage, 0, u), u, dy[u]);
-            take(slot(stage, 1, u), u, s[u]);
+            take(now[3 * u * threads], u, dy[u]);
+            take(now[(3 * u + 1) * threads], u, s[u]);
             if constexpr (!kHeld) weight_of(u, g);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -398,7 +411,7 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
         for (int u = 0; u < NU; ++u) {
             float out[N];
             if (a.dsum) {
-                unpack<T>(slot(stage, 2, u), out);
+                unpack<T>(now[(3 * u + 2) * threads], out);
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) out[i] = 0.0f;
@@ -407,7 +420,7 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
             for (int i = 0; i < N; ++i) out[i] = fmaf(-s[u][i], c, fmaf(dy[u][i], rstd, out[i]));
             if constexpr (ALIKE) {
                 const uint4 q = pack<T>(out);
-                if (whole[u]) {
+                if (all_whole || whole[u]) {
                     *reinterpret_cast<uint4*>(dx + col[u]) = q;
                 } else if (col[u] < width && col[u] + N > 0) {
                     const T* t = reinterpret_cast<const T*>(&q);
@@ -419,7 +432,8 @@ __global__ __launch_bounds__(512, NU == 1 ? 2 : 1) void norm_backward_kernel(con
                 store_unit(dx, col[u], width, pack<T>(out));
             }
         }
-        if (++stage == kDepth) stage = 0;
+        behind = now;
+        now = now == mine + (kDepth - 1) * span ? mine : now + span;
     }
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -487,29 +501,24 @@ __global__ __launch_bounds__(256) void norm_stripes_kernel(const __grid_constant
     }
 }
 
-// dweight[d] = the CTAs' partial sums in order: 8 threads a column take every
-// eighth row of `partial` each and are added in order.
-__global__ __launch_bounds__(256) void column_sum_kernel(const float* partial, int64_t pitch, int count, int64_t width,
-                                                         float* out) {
-    __shared__ float s[8][33];
-    const int64_t col = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int part = threadIdx.x >> 5;
+// dweight[d] = the CTAs' partial sums: 32 threads a column take every 32nd row
+// of `partial` each, and their sums are added in order.
+__global__ __launch_bounds__(1024) void column_sum_kernel(const float* partial, int64_t pitch, int count, int64_t width,
+                                                          float* out) {
+    __shared__ float s[32][33];
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;
     float total = 0.0f;
     if (col < width) {
-        int b = part;
-        for (; b + 24 < count; b += 32) {
-            const float v0 = partial[b * pitch + col], v1 = partial[(b + 8) * pitch + col],
-                        v2 = partial[(b + 16) * pitch + col], v3 = partial[(b + 24) * pitch + col];
-            total += (v0 + v1) + (v2 + v3);
-        }
-        for (; b < count; b += 8) total += partial[b * pitch + col];
+#pragma unroll 8
+        for (int b = part; b < count; b += 32) total += partial[b * pitch + col];
     }
-    s[part][threadIdx.x & 31] = total;
+    s[part][lane] = total;
     __syncthreads();
     if (part == 0 && col < width) {
         total = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) total += s[i][threadIdx.x & 31];
+        for (int i = 0; i < 32; ++i) total += s[i][lane];
         out[col] = total;
     }
 }
@@ -527,7 +536,9 @@ BackwardShape backward_shape(int64_t rows, int64_t width, int unit, int sms) {
     BackwardShape s{};
     s.pitch = (width + 7) / 8 * 8;
     const int64_t units = (width + unit - 1) / unit + 1;
-    s.units = units <= 512 ? 1 : units <= 1024 ? 2 : 4;
+    // two units a thread where a row has them: what a row costs beside its elements (its sum over the CTA, its
+    // addresses) is paid by half the threads (2325 bfloat16 columns: 176 -> 159 us for 40 001 rows)
+    s.units = units <= 128 ? 1 : units <= 1024 ? 2 : 4;
     if (units <= 2048) s.threads = (int)((units + s.units * 32 - 1) / (s.units * 32) * 32);
     const int64_t resident =
         s.threads ? std::max<int64_t>(1, std::min<int64_t>((s.units == 1 ? 1024 : 512) / s.threads, 16)) : 8;
@@ -564,7 +575,7 @@ void norm_backward(NormBackwardArgs<T> a, float* dweight, const BackwardShape& s
         norm_stripes_kernel<T><<<dim3((unsigned)s.grid, (unsigned)stripes), 256, 0, stream>>>(a);
     }
     check(cudaGetLastError(), "norm gradient launch");
-    column_sum_kernel<<<(unsigned)((a.s.width + 31) / 32), 256, 0, stream>>>(a.partial, s.pitch, (int)s.grid, a.s.width,
+    column_sum_kernel<<<(unsigned)((a.s.width + 31) / 32), 1024, 0, stream>>>(a.partial, s.pitch, (int)s.grid, a.s.width,
                                                                             dweight);
     check(cudaGetLastError(), "norm gradient launch");
 }

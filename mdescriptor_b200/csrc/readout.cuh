@@ -44,20 +44,53 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <class T>
 constexpr int kUnit = 16 / (int)sizeof(T);
 
+// The two 16-bit elements of a word, and back (each rounded to nearest).
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 t = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
+
 template <class T>
 __device__ __forceinline__ void unpack(const uint4& u, float (&f)[kUnit<T>]) {
-    const T* t = reinterpret_cast<const T*>(&u);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) f[i] = to_float(t[i]);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            f[i] = __uint_as_float(w[i]);
+        } else {
+            const float2 t = unpack2<T>(w[i]);
+            f[2 * i] = t.x, f[2 * i + 1] = t.y;
+        }
+    }
 }
 
 template <class T>
 __device__ __forceinline__ uint4 pack(const float (&f)[kUnit<T>]) {
-    uint4 u;
-    T* t = reinterpret_cast<T*>(&u);
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) t[i] = from_float<T>(f[i]);
-    return u;
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+        else w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Bytes [shift, shift + 16) of the 32 bytes a, b; 0 < shift < 16, the same in
@@ -173,16 +206,20 @@ struct Quad<__half> { using Word = uint2; };
 
 template <class T>
 __device__ __forceinline__ float4 unpack4(const typename Quad<T>::Word& w) {
-    const T* t = reinterpret_cast<const T*>(&w);
-    return make_float4(to_float(t[0]), to_float(t[1]), to_float(t[2]), to_float(t[3]));
+    if constexpr (sizeof(T) == 4) {
+        return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+    } else {
+        const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
 }
 
 template <class T>
 __device__ __forceinline__ typename Quad<T>::Word pack4(const float4& f) {
-    typename Quad<T>::Word w;
-    T* t = reinterpret_cast<T*>(&w);
-    t[0] = from_float<T>(f.x), t[1] = from_float<T>(f.y), t[2] = from_float<T>(f.z), t[3] = from_float<T>(f.w);
-    return w;
+    if constexpr (sizeof(T) == 4)
+        return make_uint4(__float_as_uint(f.x), __float_as_uint(f.y), __float_as_uint(f.z), __float_as_uint(f.w));
+    else
+        return make_uint2(pack2<T>(f.x, f.y), pack2<T>(f.z, f.w));
 }
 
 __device__ __forceinline__ uint2 splice(const uint2& a, const uint2& b, int shift) {
