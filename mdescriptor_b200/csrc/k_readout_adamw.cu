@@ -20,26 +20,30 @@ constexpr int kTile = kThreads * kSpan * kTileUnits;  // 4096 elements, a multip
 constexpr int kGrads = 448;                      // gradient pointers handed over in one launch's parameters
 
 struct Tensor {
-    void* p;
-    void* m;
-    void* v;
-    float* m_scale;
-    float* v_scale;
+    uint8_t *p, *m, *v;
+    float *m_scale, *v_scale;
     int64_t count;
     int64_t first;  // position in the optimizer's own numbering of elements, a multiple of 128
     float decay;    // weight decay
     int32_t vector;  // p, m and v can be read in units of four
 };
 
-struct Tile {
+// One tile: addresses of its first element, and how many it has.
+struct alignas(16) Tile {
+    uint8_t *p, *m, *v;
+    float *m_scale, *v_scale;
+    int64_t first;   // its first element in the optimizer's numbering
+    int64_t offset;  // its first element in the tensor
     int32_t tensor;
-    int32_t pad;
-    int64_t start;
+    int32_t count;
+    float decay;
+    int32_t vector;
 };
+constexpr int kTileWords = sizeof(Tile) / 4;
 
 struct StepArgs {
-    const Tensor* tensors;
     const Tile* tiles;
+    int32_t tile_count;
     int32_t first_tensor;  // of this launch: grads[0] belongs to it
     float lr, beta1, beta2, rest1, rest2, eps, step_size, root2, grad_scale;
     uint32_t key;
@@ -48,16 +52,19 @@ struct StepArgs {
 
 // Two 16-bit random numbers of an element: a counter mixed by two rounds of
 // shift, exclusive or and multiplication with odd constants (the fractional
-// parts of square roots of small primes).
-__device__ __forceinline__ uint32_t noise(int64_t element, uint32_t key) {
-    uint32_t h = (uint32_t)element ^ ((uint32_t)(element >> 32) * 0x3C6EF373u) ^ key;
+// parts of square roots of small primes).  `start`: what a quad's elements share.
+__device__ __forceinline__ uint32_t noise_start(int64_t element, uint32_t key) {
+    return (uint32_t)element ^ ((uint32_t)(element >> 32) * 0x3C6EF373u) ^ key;
+}
+__device__ __forceinline__ uint32_t noise(uint32_t start, int i) {
+    uint32_t h = start ^ i;  // a quad's first element is a multiple of four
     h = (h ^ h >> 16) * 0xA54FF53Bu;
     h = (h ^ h >> 15) * 0x510E527Fu;
     return h ^ h >> 16;
 }
 
 template <class T>
-__device__ __forceinline__ void load4(const T* p, int64_t at, int64_t count, bool vector, float (&f)[4]) {
+__device__ __forceinline__ void load4(const T* p, int at, int count, bool vector, float (&f)[4]) {
     if (vector && at + 4 <= count) {
         if constexpr (sizeof(T) == 4) {
             const float4 q = *reinterpret_cast<const float4*>(p + at);
@@ -75,7 +82,7 @@ __device__ __forceinline__ void load4(const T* p, int64_t at, int64_t count, boo
 }
 
 template <class T>
-__device__ __forceinline__ void store4(T* p, int64_t at, int64_t count, bool vector, const float (&f)[4]) {
+__device__ __forceinline__ void store4(T* p, int at, int count, bool vector, const float (&f)[4]) {
     if (vector && at + 4 <= count) {
         if constexpr (sizeof(T) == 4) {
             *reinterpret_cast<float4*>(p + at) = make_float4(f[0], f[1], f[2], f[3]);
@@ -93,7 +100,7 @@ __device__ __forceinline__ void store4(T* p, int64_t at, int64_t count, bool vec
         if (at + i < count) p[at + i] = from_float<T>(f[i]);
 }
 
-__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t at, int64_t count, bool vector) {
+__device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int at, int count, bool vector) {
     if (vector && at + 4 <= count) return *reinterpret_cast<const uint32_t*>(p + at);
     uint32_t q = 0;
 #pragma unroll
@@ -102,7 +109,7 @@ __device__ __forceinline__ uint32_t load_codes(const uint8_t* p, int64_t at, int
     return q;
 }
 
-__device__ __forceinline__ void store_codes(uint8_t* p, int64_t at, int64_t count, bool vector, uint32_t codes) {
+__device__ __forceinline__ void store_codes(uint8_t* p, int at, int count, bool vector, uint32_t codes) {
     if (vector && at + 4 <= count) {
         *reinterpret_cast<uint32_t*>(p + at) = codes;
         return;
@@ -184,7 +191,7 @@ __device__ __forceinline__ float square_root(float x) {
 template <class P, class G, bool SMALL>
 struct Update {
     const StepArgs& a;
-    const Tensor& t;
+    const Tile& t;
     const G* g;
     float keep;
 
@@ -194,21 +201,21 @@ struct Update {
         float sm, sv;
     };
 
-    __device__ __forceinline__ void load(Unit& u, int64_t at, bool vec_p, bool vec_g) const {
-        load4(static_cast<const P*>(t.p), at, t.count, vec_p, u.x);
-        load4(g, at, t.count, vec_g, u.y);
+    // `at`: the lane's first element in the tile, a multiple of four.
+    __device__ __forceinline__ void load(Unit& u, int at, int count, bool vec_p, bool vec_g) const {
+        load4(reinterpret_cast<const P*>(t.p), at, count, vec_p, u.x);
+        load4(g, at, count, vec_g, u.y);
         if constexpr (SMALL) {
-            const int64_t block = at / kBlock;  // of the warp's first lane's element: at least that one exists
-            u.qm = load_codes(static_cast<const uint8_t*>(t.m), at, t.count, vec_p);
-            u.qv = load_codes(static_cast<const uint8_t*>(t.v), at, t.count, vec_p);
-            u.sm = t.m_scale[block], u.sv = t.v_scale[block];
+            u.qm = load_codes(t.m, at, count, vec_p);
+            u.qv = load_codes(t.v, at, count, vec_p);
+            u.sm = t.m_scale[at / kBlock], u.sv = t.v_scale[at / kBlock];  // the warp's first lane has an element of it
         } else {
-            load4(static_cast<const float*>(t.m), at, t.count, vec_p, u.m);
-            load4(static_cast<const float*>(t.v), at, t.count, vec_p, u.v);
+            load4(reinterpret_cast<const float*>(t.m), at, count, vec_p, u.m);
+            load4(reinterpret_cast<const float*>(t.v), at, count, vec_p, u.v);
         }
     }
 
-    __device__ __forceinline__ void finish(Unit& u, int64_t at, bool vec_p) const {
+    __device__ __forceinline__ void finish(Unit& u, int at, int count, bool vec_p) const {
         if constexpr (SMALL) {
             decode(u.qm, u.sm, u.m);
             decode(u.qv, u.sv, u.v);
@@ -222,52 +229,68 @@ struct Update {
             const float root = fmaf(square_root(u.v[i]), a.root2, a.eps);
             u.x[i] = fmaf(-a.step_size, __fdividef(u.m[i], root), u.x[i] * keep);
         }
-        store4(static_cast<P*>(t.p), at, t.count, vec_p, u.x);
+        store4(reinterpret_cast<P*>(t.p), at, count, vec_p, u.x);
         if constexpr (SMALL) {
+            const uint32_t start = noise_start(t.first + at, a.key);
             uint32_t um[4], uv[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t h = noise(t.first + at + i, a.key);
+                const uint32_t h = noise(start, i);
                 um[i] = h >> 12 & 0xffff0u, uv[i] = h << 4 & 0xffff0u;
             }
             float sm, sv;
-            store_codes(static_cast<uint8_t*>(t.m), at, t.count, vec_p, encode<false>(u.m, um, sm));
-            store_codes(static_cast<uint8_t*>(t.v), at, t.count, vec_p, encode<true>(u.v, uv, sv));
+            store_codes(t.m, at, count, vec_p, encode<false>(u.m, um, sm));
+            store_codes(t.v, at, count, vec_p, encode<true>(u.v, uv, sv));
             if ((threadIdx.x & 31) == 0) t.m_scale[at / kBlock] = sm, t.v_scale[at / kBlock] = sv;
         } else {
-            store4(static_cast<float*>(t.m), at, t.count, vec_p, u.m);
-            store4(static_cast<float*>(t.v), at, t.count, vec_p, u.v);
+            store4(reinterpret_cast<float*>(t.m), at, count, vec_p, u.m);
+            store4(reinterpret_cast<float*>(t.v), at, count, vec_p, u.v);
         }
     }
 };
 
+// Persistent: a CTA takes tiles b, b + grid, ...; the next one's record is read
+// while this one's elements are.
 template <class P, class G, bool SMALL>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const __grid_constant__ StepArgs a) {
-    const Tile tile = a.tiles[blockIdx.x];
-    const Tensor t = a.tensors[tile.tensor];
-    const G* g = static_cast<const G*>(a.grads[tile.tensor - a.first_tensor]);
-    const Update<P, G, SMALL> update{a, t, g, 1.0f - a.lr * t.decay};
-    const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
-    const int64_t first = tile.start + threadIdx.x * kSpan;
-    if (vec_p && vec_g && tile.start + kTile <= t.count) {
-#pragma unroll
-        for (int k = 0; k < kTileUnits; k += 2) {  // two units under way
-            typename Update<P, G, SMALL>::Unit u[2];
-            const int64_t at = first + k * kThreads * kSpan;
-            update.load(u[0], at, true, true);
-            update.load(u[1], at + kThreads * kSpan, true, true);
-            update.finish(u[0], at, true);
-            update.finish(u[1], at + kThreads * kSpan, true);
-        }
-    } else {
+__global__ __launch_bounds__(kThreads, 4) void adamw_kernel(const __grid_constant__ StepArgs a) {
+    __shared__ union Record {
+        uint32_t words[kTileWords];
+        Tile tile;
+        __device__ Record() {}
+    } record[2];
+    int index = blockIdx.x;
+    if (threadIdx.x < kTileWords) record[0].words[threadIdx.x] = reinterpret_cast<const uint32_t*>(a.tiles + index)[threadIdx.x];
+    __syncthreads();
+    for (int turn = 0; index < a.tile_count; index += gridDim.x, turn ^= 1) {
+        const int next = index + gridDim.x;
+        uint32_t word = 0;
+        if (threadIdx.x < kTileWords && next < a.tile_count)
+            word = reinterpret_cast<const uint32_t*>(a.tiles + next)[threadIdx.x];
+        const Tile& t = record[turn].tile;
+        const G* g = static_cast<const G*>(a.grads[t.tensor - a.first_tensor]) + t.offset;
+        const Update<P, G, SMALL> update{a, t, g, 1.0f - a.lr * t.decay};
+        const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
+        constexpr int kAcross = kThreads * kSpan;
+        if (vec_p && vec_g && t.count == kTile) {
 #pragma unroll 1
-        for (int k = 0; k < kTileUnits; ++k) {
-            const int64_t at = first + k * kThreads * kSpan;
-            if (at - (threadIdx.x & 31) * kSpan >= t.count) break;  // the whole warp
-            typename Update<P, G, SMALL>::Unit u;
-            update.load(u, at, vec_p, vec_g);
-            update.finish(u, at, vec_p);
+            for (int at = threadIdx.x * kSpan; at < kTile; at += 2 * kAcross) {  // two units under way
+                typename Update<P, G, SMALL>::Unit u[2];
+                update.load(u[0], at, kTile, true, true);
+                update.load(u[1], at + kAcross, kTile, true, true);
+                update.finish(u[0], at, kTile, true);
+                update.finish(u[1], at + kAcross, kTile, true);
+            }
+        } else {
+            const int count = t.count;
+#pragma unroll 1
+            for (int at = threadIdx.x * kSpan; at - (int)(threadIdx.x & 31) * kSpan < count; at += kAcross) {  // by warps
+                typename Update<P, G, SMALL>::Unit u;
+                update.load(u, at, count, vec_p, vec_g);
+                update.finish(u, at, count, vec_p);
+            }
         }
+        if (threadIdx.x < kTileWords) record[turn ^ 1].words[threadIdx.x] = word;
+        __syncthreads();
     }
 }
 
@@ -279,7 +302,7 @@ struct mdsoap_adamw {
     std::vector<int64_t> tile_begin;  // [tensors + 1]
     int32_t dtype = 0, state_bits = 32, device = 0;
     uint32_t seed = 0;
-    void* table = nullptr;  // tensors, then tiles, on `device`
+    void* table = nullptr;  // the tiles, on `device`
     ~mdsoap_adamw() {
         if (table) cudaFree(table);
     }
@@ -287,28 +310,39 @@ struct mdsoap_adamw {
 
 namespace {
 
-// The table of tensors and tiles on the device, uploaded by the first step.
+// The table of tiles on the device, uploaded by the first step.
 void upload(mdsoap_adamw& o) {
     if (o.table) return;
-    const int64_t tiles = o.tile_begin.back();
-    const size_t head = o.tensors.size() * sizeof(Tensor);
-    std::vector<unsigned char> host(head + tiles * sizeof(Tile));
-    std::copy_n(reinterpret_cast<const unsigned char*>(o.tensors.data()), head, host.data());
-    Tile* tile = reinterpret_cast<Tile*>(host.data() + head);
-    for (size_t i = 0; i < o.tensors.size(); ++i)
-        for (int64_t k = 0; k < o.tile_begin[i + 1] - o.tile_begin[i]; ++k) *tile++ = {(int32_t)i, 0, k * kTile};
+    std::vector<Tile> host(o.tile_begin.back());
+    Tile* tile = host.data();
+    const int64_t p_size = o.dtype == MDSOAP_FLOAT32 ? 4 : 2, state_size = o.state_bits / 8;
+    for (size_t i = 0; i < o.tensors.size(); ++i) {
+        const Tensor& t = o.tensors[i];
+        for (int64_t at = 0; at < t.count; at += kTile)
+            *tile++ = {t.p + at * p_size,
+                       t.m + at * state_size,
+                       t.v + at * state_size,
+                       t.m_scale ? t.m_scale + at / kBlock : nullptr,
+                       t.v_scale ? t.v_scale + at / kBlock : nullptr,
+                       t.first + at,
+                       at,
+                       (int32_t)i,
+                       (int32_t)std::min<int64_t>(kTile, t.count - at),
+                       t.decay,
+                       t.vector};
+    }
     void* table = nullptr;
-    check(engine_malloc(&table, host.size()), "optimizer table");
-    const cudaError_t err = cudaMemcpy(table, host.data(), host.size(), cudaMemcpyHostToDevice);
+    check(engine_malloc(&table, host.size() * sizeof(Tile)), "optimizer table");
+    const cudaError_t err = cudaMemcpy(table, host.data(), host.size() * sizeof(Tile), cudaMemcpyHostToDevice);
     if (err != cudaSuccess) cudaFree(table);
     check(err, "optimizer table upload");
     o.table = table;
 }
 
 template <class P, class G>
-void launch(bool small, const StepArgs& a, unsigned tiles, cudaStream_t stream) {
-    if (small) adamw_kernel<P, G, true><<<tiles, kThreads, 0, stream>>>(a);
-    else adamw_kernel<P, G, false><<<tiles, kThreads, 0, stream>>>(a);
+void launch(bool small, const StepArgs& a, unsigned grid, cudaStream_t stream) {
+    if (small) adamw_kernel<P, G, true><<<grid, kThreads, 0, stream>>>(a);
+    else adamw_kernel<P, G, false><<<grid, kThreads, 0, stream>>>(a);
     check(cudaGetLastError(), "optimizer launch");
 }
 
@@ -339,9 +373,9 @@ int mdsoap_adamw_create(const mdsoap_adamw_params* params, mdsoap_adamw** optimi
             Tensor t{};
             t.count = q.counts[i];
             need(t.count >= 0, "readout: negative tensor size");
-            t.p = q.params[i];
-            t.m = q.exp_avg[i];
-            t.v = q.exp_avg_sq[i];
+            t.p = static_cast<uint8_t*>(q.params[i]);
+            t.m = static_cast<uint8_t*>(q.exp_avg[i]);
+            t.v = static_cast<uint8_t*>(q.exp_avg_sq[i]);
             if (q.state_bits == 8) t.m_scale = q.exp_avg_scale[i], t.v_scale = q.exp_avg_sq_scale[i];
             need(t.count == 0 || (t.p && t.m && t.v && (q.state_bits == 32 || (t.m_scale && t.v_scale))),
                  "readout: null optimizer tensor");
@@ -379,9 +413,8 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         check(cudaSetDevice(o.device), "cudaSetDevice");
         upload(o);
         StepArgs a;
-        a.tensors = static_cast<const Tensor*>(o.table);
-        const Tile* tiles =
-            reinterpret_cast<const Tile*>(static_cast<const unsigned char*>(o.table) + o.tensors.size() * sizeof(Tensor));
+        const Tile* tiles = static_cast<const Tile*>(o.table);
+        const int sms = sm_count(o.device);
         a.lr = (float)lr;
         a.beta1 = (float)beta1;
         a.beta2 = (float)beta2;
@@ -397,11 +430,12 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
             const int64_t count = o.tile_begin[end] - o.tile_begin[i];
             if (count == 0) continue;
             a.first_tensor = (int32_t)i;
+            a.tile_count = (int32_t)count;
             a.tiles = tiles + o.tile_begin[i];
             std::copy(grads + i, grads + end, a.grads);
             by_type(o.dtype, [&](auto p) {
                 by_type(grad_dtype, [&](auto g) {
-                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)count,
+                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)std::min<int64_t>(count, 4 * sms),
                                                      static_cast<cudaStream_t>(stream));
                 });
             });
