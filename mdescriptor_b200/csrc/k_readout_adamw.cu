@@ -128,18 +128,30 @@ __device__ __forceinline__ void decode(uint32_t codes, float scale, float (&f)[4
     }
 }
 
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float square_root(float x) {
+    float r;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // Codes of four values of the warp's block of 128, and the block's scale.
 // a = |x| / scale (at most 448) goes down to an e4m3 value after u / 2^16 of
 // that value's step has been added; `u20` holds the u, times 16.  From 2^-6 on
 // the step is bit 20 of the float, so the sum's top bits are the code; below it
 // is 2^-9 (rare: the warp looks whether it has such values at all).  The
-// quotient is x times the rounded reciprocal with one correction (Markstein's
-// method).  FLOOR: a positive x keeps at least the smallest code.
+// quotient is x times the approximate reciprocal with one correction by the
+// exact remainder, which leaves the correctly rounded one but for about one in a
+// million.  FLOOR: a positive x keeps at least the smallest code.
 template <bool FLOOR>
 __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&u20)[4], float& scale) {
     const float top = warp_larger(larger(larger(x[0], x[1], x[2]), x[3]));
     scale = top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop);
-    const float inverse = __frcp_rn(scale);
+    const float inverse = reciprocal(scale);
     float a[4], least = kTop;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -169,16 +181,11 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
     return scale == 0.0f ? 0u : codes;
 }
 
-__device__ __forceinline__ float square_root(float x) {
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 // One CTA a tile of 4096 elements of one tensor.
 //   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// in float32, each stored value rounded once.
+// in float32, each stored value rounded once; root and quotient of p's update are
+// the quick ones (2^-22 of the update).
 // 8-bit states are e4m3 codes with a float32 scale for each block of 128
 // elements of the tensor; a warp holds exactly one block at a time.  They are
 // rounded by dithering: b2 = 0.999 moves v by a thousandth a step and the codes
@@ -226,8 +233,9 @@ struct Update {
             // products rounded, then the sum: the states' codes depend on every bit of it
             u.m[i] = __fadd_rn(__fmul_rn(a.beta1, u.m[i]), __fmul_rn(a.rest1, grad));
             u.v[i] = __fadd_rn(__fmul_rn(a.beta2, u.v[i]), __fmul_rn(__fmul_rn(a.rest2, grad), grad));
-            const float root = fmaf(square_root(u.v[i]), a.root2, a.eps);
-            u.x[i] = fmaf(-a.step_size, __fdividef(u.m[i], root), u.x[i] * keep);
+            // 2^24 keeps the smallest v out of the root's flush to zero (root2 holds its 2^-12)
+            const float root = fmaf(square_root(u.v[i] * 0x1p24f), a.root2, a.eps);
+            u.x[i] = fmaf(-a.step_size, u.m[i] * reciprocal(root), u.x[i] * keep);
         }
         store4(reinterpret_cast<P*>(t.p), at, count, vec_p, u.x);
         if constexpr (SMALL) {
@@ -249,47 +257,70 @@ struct Update {
     }
 };
 
-// Persistent: a CTA takes tiles b, b + grid, ...; the next one's record is read
-// while this one's elements are.
+// Persistent: a CTA takes tiles b, b + grid, ...; records are read two tiles
+// ahead, elements half a tile (two units a thread) ahead.
 template <class P, class G, bool SMALL>
-__global__ __launch_bounds__(kThreads, 4) void adamw_kernel(const __grid_constant__ StepArgs a) {
+__global__ __launch_bounds__(kThreads, 3) void adamw_kernel(const __grid_constant__ StepArgs a) {
     __shared__ union Record {
         uint32_t words[kTileWords];
         Tile tile;
         __device__ Record() {}
-    } record[2];
+    } record[3];
+    constexpr int kAcross = kThreads * kSpan, kHalf = 2 * kAcross;
+    using Work = Update<P, G, SMALL>;
+    const int step = gridDim.x, mine = threadIdx.x * kSpan;
     int index = blockIdx.x;
-    if (threadIdx.x < kTileWords) record[0].words[threadIdx.x] = reinterpret_cast<const uint32_t*>(a.tiles + index)[threadIdx.x];
+    const auto word_of = [&](int tile) {
+        return threadIdx.x < kTileWords && tile < a.tile_count
+                   ? reinterpret_cast<const uint32_t*>(a.tiles + tile)[threadIdx.x]
+                   : 0u;
+    };
+    const auto grad_of = [&](const Tile& t) { return static_cast<const G*>(a.grads[t.tensor - a.first_tensor]) + t.offset; };
+    const auto plain = [&](const Tile& t) {  // full and aligned
+        return t.count == kTile && t.vector && reinterpret_cast<uintptr_t>(grad_of(t)) % (4 * sizeof(G)) == 0;
+    };
+    if (threadIdx.x < kTileWords) {
+        record[0].words[threadIdx.x] = word_of(index);
+        record[1].words[threadIdx.x] = word_of(index + step);
+    }
     __syncthreads();
-    for (int turn = 0; index < a.tile_count; index += gridDim.x, turn ^= 1) {
-        const int next = index + gridDim.x;
-        uint32_t word = 0;
-        if (threadIdx.x < kTileWords && next < a.tile_count)
-            word = reinterpret_cast<const uint32_t*>(a.tiles + next)[threadIdx.x];
+    typename Work::Unit u[2], v[2];
+    bool ready = false;  // u holds this tile's first half
+    for (int turn = 0; index < a.tile_count; index += step) {
+        const uint32_t word = word_of(index + 2 * step);
         const Tile& t = record[turn].tile;
-        const G* g = static_cast<const G*>(a.grads[t.tensor - a.first_tensor]) + t.offset;
-        const Update<P, G, SMALL> update{a, t, g, 1.0f - a.lr * t.decay};
-        const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(g) % (4 * sizeof(G)) == 0;
-        constexpr int kAcross = kThreads * kSpan;
-        if (vec_p && vec_g && t.count == kTile) {
-#pragma unroll 1
-            for (int at = threadIdx.x * kSpan; at < kTile; at += 2 * kAcross) {  // two units under way
-                typename Update<P, G, SMALL>::Unit u[2];
-                update.load(u[0], at, kTile, true, true);
-                update.load(u[1], at + kAcross, kTile, true, true);
-                update.finish(u[0], at, kTile, true);
-                update.finish(u[1], at + kAcross, kTile, true);
+        const int next = turn == 2 ? 0 : turn + 1;
+        const Work work{a, t, grad_of(t), 1.0f - a.lr * t.decay};
+        if (plain(t)) {
+            if (!ready) {
+                work.load(u[0], mine, kTile, true, true);
+                work.load(u[1], mine + kAcross, kTile, true, true);
             }
+            work.load(v[0], mine + kHalf, kTile, true, true);
+            work.load(v[1], mine + kHalf + kAcross, kTile, true, true);
+            work.finish(u[0], mine, kTile, true);
+            work.finish(u[1], mine + kAcross, kTile, true);
+            const Tile& n = record[next].tile;
+            ready = index + step < a.tile_count && plain(n);
+            if (ready) {
+                const Work ahead{a, n, grad_of(n), 0.0f};
+                ahead.load(u[0], mine, kTile, true, true);
+                ahead.load(u[1], mine + kAcross, kTile, true, true);
+            }
+            work.finish(v[0], mine + kHalf, kTile, true);
+            work.finish(v[1], mine + kHalf + kAcross, kTile, true);
         } else {
             const int count = t.count;
+            const bool vec_p = t.vector, vec_g = reinterpret_cast<uintptr_t>(work.g) % (4 * sizeof(G)) == 0;
+            ready = false;
 #pragma unroll 1
-            for (int at = threadIdx.x * kSpan; at - (int)(threadIdx.x & 31) * kSpan < count; at += kAcross) {  // by warps
-                typename Update<P, G, SMALL>::Unit u;
-                update.load(u, at, count, vec_p, vec_g);
-                update.finish(u, at, count, vec_p);
+            for (int at = mine; at - (int)(threadIdx.x & 31) * kSpan < count; at += kAcross) {  // by warps
+                work.load(u[0], at, count, vec_p, vec_g);
+                work.finish(u[0], at, count, vec_p);
             }
         }
-        if (threadIdx.x < kTileWords) record[turn ^ 1].words[threadIdx.x] = word;
+        if (threadIdx.x < kTileWords) record[next == 2 ? 0 : next + 1].words[threadIdx.x] = word;
+        turn = next;
         __syncthreads();
     }
 }
@@ -422,7 +453,7 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         a.rest2 = (float)(1.0 - beta2);
         a.eps = (float)eps;
         a.step_size = (float)(lr / (1.0 - std::pow(beta1, (double)step)));
-        a.root2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
+        a.root2 = (float)(0x1p-12 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
         a.grad_scale = (float)grad_scale;
         a.key = o.seed * 0x6A09E667u + (uint32_t)step * 0xBB67AE85u;
         for (size_t i = 0; i < o.tensors.size(); i += kGrads) {
@@ -435,7 +466,7 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
             std::copy(grads + i, grads + end, a.grads);
             by_type(o.dtype, [&](auto p) {
                 by_type(grad_dtype, [&](auto g) {
-                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)std::min<int64_t>(count, 4 * sms),
+                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)std::min<int64_t>(count, 3 * sms),
                                                      static_cast<cudaStream_t>(stream));
                 });
             });
