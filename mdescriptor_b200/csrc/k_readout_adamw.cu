@@ -334,6 +334,7 @@ struct mdsoap_adamw {
     int32_t dtype = 0, state_bits = 32, device = 0;
     uint32_t seed = 0;
     void* table = nullptr;  // the tiles, on `device`
+    bool ready = false;     // the table holds them
     ~mdsoap_adamw() {
         if (table) cudaFree(table);
     }
@@ -341,33 +342,53 @@ struct mdsoap_adamw {
 
 namespace {
 
-// The table of tiles on the device, uploaded by the first step.
-void upload(mdsoap_adamw& o) {
-    if (o.table) return;
-    std::vector<Tile> host(o.tile_begin.back());
-    Tile* tile = host.data();
-    const int64_t p_size = o.dtype == MDSOAP_FLOAT32 ? 4 : 2, state_size = o.state_bits / 8;
-    for (size_t i = 0; i < o.tensors.size(); ++i) {
-        const Tensor& t = o.tensors[i];
-        for (int64_t at = 0; at < t.count; at += kTile)
-            *tile++ = {t.p + at * p_size,
-                       t.m + at * state_size,
-                       t.v + at * state_size,
-                       t.m_scale ? t.m_scale + at / kBlock : nullptr,
-                       t.v_scale ? t.v_scale + at / kBlock : nullptr,
-                       t.first + at,
-                       at,
-                       (int32_t)i,
-                       (int32_t)std::min<int64_t>(kTile, t.count - at),
-                       t.decay,
-                       t.vector};
+// Tile records from the tensors and their first tiles ([tensors + 1]).
+__global__ void tiles_kernel(const Tensor* tensors, const int64_t* begin, int count, int p_size, int state_size, Tile* out) {
+    const int64_t index = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (index >= begin[count]) return;
+    int low = 0, high = count;  // the last tensor that begins at or before this tile and has tiles
+    while (high - low > 1) {
+        const int middle = (low + high) / 2;
+        if (begin[middle] <= index) low = middle;
+        else high = middle;
     }
+    const Tensor t = tensors[low];
+    const int64_t at = (index - begin[low]) * kTile;
+    out[index] = {t.p + at * p_size,
+                  t.m + at * state_size,
+                  t.v + at * state_size,
+                  t.m_scale ? t.m_scale + at / kBlock : nullptr,
+                  t.v_scale ? t.v_scale + at / kBlock : nullptr,
+                  t.first + at,
+                  at,
+                  low,
+                  (int32_t)min((int64_t)kTile, t.count - at),
+                  t.decay,
+                  t.vector};
+}
+
+// The table of tiles on the device, made by the first step on its stream.
+void upload(mdsoap_adamw& o, cudaStream_t stream) {
+    if (o.ready) return;
+    if (o.table) cudaFree(o.table), o.table = nullptr;  // of an upload that failed
+    const int64_t tiles = o.tile_begin.back();
+    const size_t records = tiles * sizeof(Tile), tensors = o.tensors.size() * sizeof(Tensor);
     void* table = nullptr;
-    check(engine_malloc(&table, host.size() * sizeof(Tile)), "optimizer table");
-    const cudaError_t err = cudaMemcpy(table, host.data(), host.size() * sizeof(Tile), cudaMemcpyHostToDevice);
-    if (err != cudaSuccess) cudaFree(table);
-    check(err, "optimizer table upload");
-    o.table = table;
+    check(engine_malloc(&table, records + tensors + o.tile_begin.size() * sizeof(int64_t)), "optimizer table");
+    o.table = table;  // freed with the optimizer
+    uint8_t* const device = static_cast<uint8_t*>(table);
+    const auto put = [&](size_t at, const void* from, size_t bytes) {
+        check(cudaMemcpyAsync(device + at, from, bytes, cudaMemcpyHostToDevice, stream), "optimizer table upload");
+    };
+    put(records, o.tensors.data(), tensors);  // pageable: copied out before the call returns
+    put(records + tensors, o.tile_begin.data(), o.tile_begin.size() * sizeof(int64_t));
+    tiles_kernel<<<(unsigned)((tiles + 127) / 128), 128, 0, stream>>>(
+        reinterpret_cast<const Tensor*>(device + records), reinterpret_cast<const int64_t*>(device + records + tensors),
+        (int)o.tensors.size(), o.dtype == MDSOAP_FLOAT32 ? 4 : 2, o.state_bits / 8, reinterpret_cast<Tile*>(device));
+    check(cudaGetLastError(), "optimizer table launch");
+    // later steps may come on other streams
+    check(cudaStreamSynchronize(stream), "optimizer table");
+    o.ready = true;
 }
 
 template <class P, class G>
@@ -442,7 +463,7 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         if (o.tile_begin.back() == 0) return;
         std::lock_guard<std::mutex> lock(o.mutex);
         check(cudaSetDevice(o.device), "cudaSetDevice");
-        upload(o);
+        upload(o, static_cast<cudaStream_t>(stream));
         StepArgs a;
         const Tile* tiles = static_cast<const Tile*>(o.table);
         const int sms = sm_count(o.device);
