@@ -23,7 +23,9 @@ One layer y = rms_norm(x + r) W^T and its gradients::
 from __future__ import annotations
 
 import ctypes
+from array import array
 from functools import lru_cache
+from operator import attrgetter
 from typing import NamedTuple, Sequence
 
 import torch
@@ -36,6 +38,7 @@ BLOCK = 128
 _DTYPES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
 _NAMES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 _CODES = torch.float8_e4m3fn
+_dtype_of = attrgetter("dtype")
 
 
 class Blocks(NamedTuple):
@@ -72,23 +75,26 @@ class Norm(NamedTuple):
     rstd: torch.Tensor
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The handle of a device's current stream, without the Stream object around it.
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _matrix(x: torch.Tensor, name: str) -> tuple[int, int, int]:
     """(rows, width, row pitch) of a 2-D CUDA tensor with unit column stride."""
-    if x.dim() != 2:
-        raise ValueError(f"{name} must have two dimensions, got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name} must have two dimensions, got {tuple(shape)}")
     if not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    rows, width = x.shape
+    rows, width = shape
     stride, unit = x.stride()
     if unit != 1 and width > 1:
         raise ValueError(f"{name} must have unit column stride, got strides {x.stride()}")
-    if rows > 1 and stride < width:
-        raise ValueError(f"{name} has rows that overlap (strides {x.stride()})")
-    return rows, width, max(stride, width)
+    if stride < width:
+        if rows > 1:
+            raise ValueError(f"{name} has rows that overlap (strides {x.stride()})")
+        stride = width
+    return rows, width, stride
 
 
 def _dtype(x: torch.Tensor, name: str) -> int:
@@ -98,28 +104,28 @@ def _dtype(x: torch.Tensor, name: str) -> int:
     return code
 
 
-def _vector(x: torch.Tensor | None, count: int, like: torch.Tensor, name: str) -> int | None:
+def _vector(x: torch.Tensor | None, count: int, device: int, name: str) -> int | None:
     if x is None:
         return None
-    if x.dtype != torch.float32 or x.shape != (count,) or not x.is_contiguous() or x.device != like.device:
-        raise ValueError(f"{name} must be a contiguous float32 vector of {count} on {like.device}")
+    if x.dtype != torch.float32 or x.shape != (count,) or not x.is_contiguous() or x.get_device() != device:
+        raise ValueError(f"{name} must be a contiguous float32 vector of {count} on CUDA device {device}")
     return x.data_ptr()
 
 
 def _same(x: torch.Tensor, like: torch.Tensor, name: str) -> int:
     """Row pitch of a matrix with the shape, type and device of ``like``."""
-    if x.shape != like.shape or x.dtype != like.dtype or x.device != like.device:
+    if x.shape != like.shape or x.dtype != like.dtype or x.get_device() != like.get_device():
         raise ValueError(f"{name} must have shape {tuple(like.shape)}, type {like.dtype} and device {like.device}")
     return _matrix(x, name)[2]
 
 
-def _empty_blocks(rows: int, width: int, scale_rows: int, device: torch.device) -> Blocks:
+def _empty_blocks(rows: int, width: int, scale_rows: int, device: torch.device) -> tuple[Blocks, int, int]:
+    """New blocks, with their row pitch and scale pitch."""
     blocks = (width + BLOCK - 1) // BLOCK
     pitch, scale_pitch = (width + 15) // 16 * 16, (blocks + 3) // 4 * 4
-    values = torch.empty((rows, pitch), dtype=_CODES, device=device)
-    scales = torch.empty((scale_rows, scale_pitch), dtype=torch.float32, device=device)
-    return Blocks(values if pitch == width else values[:, :width],
-                  scales if scale_pitch == blocks else scales[:, :blocks])
+    return Blocks(torch.empty_strided((rows, width), (pitch, 1), dtype=_CODES, device=device),
+                  torch.empty_strided((scale_rows, blocks), (scale_pitch, 1), dtype=torch.float32, device=device)
+                  ), pitch, scale_pitch
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -133,23 +139,25 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
         raise ValueError("output must be None or 'float8'")
     rows, width, stride = _matrix(x, "x")
     dtype = _dtype(x, "x")
-    weight_ptr = _vector(weight, width, x, "weight")
-    residual_stride = 0 if residual is None else _same(residual, x, "residual")
-    total = x if residual is None else torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    device, index = x.device, x.get_device()
+    weight_ptr = _vector(weight, width, index, "weight")
+    if residual is None:
+        total, residual_ptr, residual_stride, sum_ptr = x, None, 0, None
+    else:
+        residual_stride = _same(residual, x, "residual")
+        total = torch.empty_strided((rows, width), (width, 1), dtype=x.dtype, device=device)
+        residual_ptr, sum_ptr = residual.data_ptr(), total.data_ptr()
+    rstd = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device)
     if output is None:
-        out: Blocks | torch.Tensor = torch.empty((rows, width), dtype=x.dtype, device=x.device)
+        out: Blocks | torch.Tensor = torch.empty_strided((rows, width), (width, 1), dtype=x.dtype, device=device)
         out_ptr, out_stride, scales_ptr, scale_stride = out.data_ptr(), width, None, 0
     else:
-        out = _empty_blocks(rows, width, rows, x.device)
-        out_ptr, out_stride = out.values.data_ptr(), out.values.stride(0)
-        scales_ptr, scale_stride = out.scales.data_ptr(), out.scales.stride(0)
-        if rows == 0 or width == 0:
-            scales_ptr = scales_ptr or 16  # no element is touched; the form stays 8-bit
-    raise_for(lib.mdsoap_rms_norm(
-        x.data_ptr(), rows, width, stride, None if residual is None else residual.data_ptr(), residual_stride, dtype,
-        weight_ptr, eps, None if residual is None else total.data_ptr(), width, rstd.data_ptr(), out_ptr, out_stride,
-        scales_ptr, scale_stride, x.device.index, _stream(x.device.index)))
+        out, out_stride, scale_stride = _empty_blocks(rows, width, rows, device)
+        out_ptr, scales_ptr = out.values.data_ptr(), out.scales.data_ptr()
+    if rows and width:
+        raise_for(lib.mdsoap_rms_norm(
+            x.data_ptr(), rows, width, stride, residual_ptr, residual_stride, dtype, weight_ptr, eps, sum_ptr, width,
+            rstd.data_ptr(), out_ptr, out_stride, scales_ptr, scale_stride, index, _stream(index)))
     return Norm(out, total, rstd)
 
 
@@ -172,9 +180,9 @@ def rms_norm_backward(dy: torch.Tensor, sum: torch.Tensor, rstd: torch.Tensor, w
     dtype = _dtype(sum, "sum")
     dy_stride = _same(dy, sum, "dy")
     dsum_stride = 0 if dsum is None else _same(dsum, sum, "dsum")
-    rstd_ptr = _vector(rstd, rows, sum, "rstd")
-    weight_ptr = _vector(weight, width, sum, "weight")
-    device = sum.device.index
+    device = sum.get_device()
+    rstd_ptr = _vector(rstd, rows, device, "rstd")
+    weight_ptr = _vector(weight, width, device, "weight")
     bytes_ = _norm_backward_bytes(rows, width, dtype, device)
     dx = torch.empty((rows, width), dtype=sum.dtype, device=sum.device)
     dweight = torch.empty(width, dtype=torch.float32, device=sum.device)
@@ -197,24 +205,25 @@ def quantize(x: torch.Tensor, layout: str = "rows", row_factor: torch.Tensor | N
         raise ValueError("layout must be 'rows', 'columns', 'both' or 'tiles'")
     rows, width, stride = _matrix(x, "x")
     dtype = _dtype(x, "x")
-    row_ptr = _vector(row_factor, rows, x, "row_factor")
-    col_ptr = _vector(col_factor, width, x, "col_factor")
+    device, index = x.device, x.get_device()
+    row_ptr = _vector(row_factor, rows, index, "row_factor")
+    col_ptr = _vector(col_factor, width, index, "col_factor")
     tiles = layout == "tiles"
     if tiles and (row_ptr or col_ptr):
         raise ValueError("tiles take no factors")
-    by_rows = by_columns = None
-    args: list = [None, 0, None, 0, None, 0, None, 0]
+    by_rows = by_columns = codes = scales = codes_t = scales_t = None
+    pitch = scale_pitch = pitch_t = scale_pitch_t = 0
     if layout != "columns":
-        by_rows = _empty_blocks(rows, width, (rows + BLOCK - 1) // BLOCK if tiles else rows, x.device)
-        args[:4] = (by_rows.values.data_ptr(), by_rows.values.stride(0), by_rows.scales.data_ptr(),
-                    by_rows.scales.stride(0))
+        by_rows, pitch, scale_pitch = _empty_blocks(rows, width, (rows + BLOCK - 1) // BLOCK if tiles else rows, device)
+        codes, scales = by_rows.values.data_ptr(), by_rows.scales.data_ptr()
     if layout != "rows":
-        by_columns = _empty_blocks(width, rows, (width + BLOCK - 1) // BLOCK if tiles else width, x.device)
-        args[4:] = (by_columns.values.data_ptr(), by_columns.values.stride(0), by_columns.scales.data_ptr(),
-                    by_columns.scales.stride(0))
+        by_columns, pitch_t, scale_pitch_t = _empty_blocks(width, rows, (width + BLOCK - 1) // BLOCK if tiles else width,
+                                                           device)
+        codes_t, scales_t = by_columns.values.data_ptr(), by_columns.scales.data_ptr()
     if rows and width:
-        raise_for(lib.mdsoap_quantize(x.data_ptr(), rows, width, stride, dtype, row_ptr, col_ptr, int(tiles), *args,
-                                      x.device.index, _stream(x.device.index)))
+        raise_for(lib.mdsoap_quantize(x.data_ptr(), rows, width, stride, dtype, row_ptr, col_ptr, tiles, codes, pitch,
+                                      scales, scale_pitch, codes_t, pitch_t, scales_t, scale_pitch_t, index,
+                                      _stream(index)))
     return Quantized(by_rows, by_columns)
 
 
@@ -225,7 +234,7 @@ def _blocks(b: Blocks, name: str, tiles: bool) -> tuple[int, int, int, int, bool
     if values.dtype != _CODES:
         raise ValueError(f"{name}.values must be float8_e4m3fn, got {values.dtype}")
     scale_rows, blocks, scale_stride = _matrix(scales, f"{name}.scales")
-    if scales.dtype != torch.float32 or scales.device != values.device:
+    if scales.dtype != torch.float32 or scales.get_device() != values.get_device():
         raise ValueError(f"{name}.scales must be float32 on {values.device}")
     by_rows = scale_rows == rows
     if blocks != (width + BLOCK - 1) // BLOCK or not (by_rows or (tiles and scale_rows == (rows + BLOCK - 1) // BLOCK)):
@@ -253,28 +262,30 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
     n, k_b, b_stride, b_scale_stride, tiles = _blocks(b, "b", True)
     if k != k_b:
         raise ValueError(f"a and b must have the same width, got {k} and {k_b}")
-    device = a.values.device
-    if b.values.device != device:
+    device, index = a.values.device, a.values.get_device()
+    if b.values.get_device() != index:
         raise ValueError("a and b must be on the same device")
     if out is None:
-        if dtype not in ("bfloat16", "float32"):
+        kind = _NAMES.get(dtype)
+        if kind is None or kind is torch.float16:
             raise ValueError("dtype must be 'bfloat16' or 'float32'")
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((m, n), dtype=_NAMES[dtype], device=device)
+        out = torch.empty_strided((m, n), (n, 1), dtype=kind, device=device)
         out_stride = n
     else:
-        if out.shape != (m, n) or out.device != device or out.dtype not in (torch.bfloat16, torch.float32):
+        kind = out.dtype
+        if out.shape != (m, n) or out.get_device() != index or kind not in (torch.bfloat16, torch.float32):
             raise ValueError(f"out must be a bfloat16 or float32 matrix of shape {(m, n)} on {device}")
         out_stride = _matrix(out, "out")[2]
-        if accumulate and out.dtype != torch.float32:
+        if accumulate and kind != torch.float32:
             raise ValueError("accumulate needs a float32 out")
-    bytes_ = _matmul_bytes(m, n, k, tiles, device.index)
+    bytes_ = _matmul_bytes(m, n, k, tiles, index)
     workspace = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
     raise_for(lib.mdsoap_matmul(
         a.values.data_ptr(), m, a_stride, a.scales.data_ptr(), a_scale_stride, b.values.data_ptr(), n, b_stride,
-        b.scales.data_ptr(), b_scale_stride, int(tiles), k, _DTYPES[out.dtype], int(accumulate), out.data_ptr(),
-        out_stride, None if workspace is None else workspace.data_ptr(), bytes_, device.index, _stream(device.index)))
+        b.scales.data_ptr(), b_scale_stride, tiles, k, _DTYPES[kind], accumulate, out.data_ptr(), out_stride,
+        None if workspace is None else workspace.data_ptr(), bytes_, index, _stream(index)))
     return out
 
 
@@ -350,16 +361,16 @@ class AdamW:
     def step(self, grads: Sequence[torch.Tensor], lr: float | None = None, grad_scale: float = 1.0) -> None:
         """Update every tensor with its gradient (one type for all, times ``grad_scale``)."""
         grads = list(grads)
-        if [g.numel() for g in grads] != self._counts:
+        if list(map(torch.Tensor.numel, grads)) != self._counts:
             raise ValueError("grads must be one tensor for each of params, of its size")
-        dtype = grads[0].dtype
-        if any(g.dtype != dtype or not g.is_contiguous() or g.device != self.device for g in grads):
+        if (len(set(map(_dtype_of, grads))) != 1 or not all(map(torch.Tensor.is_contiguous, grads))
+                or set(map(torch.Tensor.get_device, grads)) != {self.device.index}):
             raise ValueError(f"grads must be contiguous tensors of one type on {self.device}")
         step = self.state["step"] + 1
+        pointers = array("Q", map(torch.Tensor.data_ptr, grads))
         raise_for(lib.mdsoap_adamw_step(
-            self._optimizer, (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads]), _dtype(grads[0], "grads"),
-            step, self.lr if lr is None else lr, self.betas[0], self.betas[1], self.eps, grad_scale,
-            _stream(self.device.index)))
+            self._optimizer, pointers.buffer_info()[0], _dtype(grads[0], "grads"), step, self.lr if lr is None else lr,
+            self.betas[0], self.betas[1], self.eps, grad_scale, _stream(self.device.index)))
         self.state["step"] = step
 
     def close(self) -> None:
