@@ -18,6 +18,7 @@ constexpr int kSpan = 4;                         // elements of one thread's uni
 constexpr int kTileUnits = 4;                    // units of a thread in one tile
 constexpr int kTile = kThreads * kSpan * kTileUnits;  // 4096 elements, a multiple of the block of 128
 constexpr int kGrads = 448;                      // gradient pointers handed over in one launch's parameters
+constexpr int kFewGrads = 24;
 
 struct Tensor {
     uint8_t *p, *m, *v;
@@ -41,13 +42,17 @@ struct alignas(16) Tile {
 };
 constexpr int kTileWords = sizeof(Tile) / 4;
 
-struct StepArgs {
+struct StepSettings {
     const Tile* tiles;
     int32_t tile_count;
     int32_t first_tensor;  // of this launch: grads[0] belongs to it
     float lr, beta1, beta2, rest1, rest2, eps, step_size, root2, grad_scale;
     uint32_t key;
-    const void* grads[kGrads];
+};
+// A launch's parameters are copied with it: few gradients take a short form.
+template <int GRADS>
+struct StepArgs : StepSettings {
+    const void* grads[GRADS];
 };
 
 // Two 16-bit random numbers of an element: a counter mixed by two rounds of
@@ -197,7 +202,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 // Bound by HBM: p, m, v in and out, g in.
 template <class P, class G, bool SMALL>
 struct Update {
-    const StepArgs& a;
+    const StepSettings& a;
     const Tile& t;
     const G* g;
     float keep;
@@ -259,8 +264,8 @@ struct Update {
 
 // Persistent: a CTA takes tiles b, b + grid, ...; records are read two tiles
 // ahead, elements half a tile (two units a thread) ahead.
-template <class P, class G, bool SMALL>
-__global__ __launch_bounds__(kThreads, 3) void adamw_kernel(const __grid_constant__ StepArgs a) {
+template <class P, class G, bool SMALL, int GRADS>
+__global__ __launch_bounds__(kThreads, 3) void adamw_kernel(const __grid_constant__ StepArgs<GRADS> a) {
     __shared__ union Record {
         uint32_t words[kTileWords];
         Tile tile;
@@ -391,10 +396,14 @@ void upload(mdsoap_adamw& o, cudaStream_t stream) {
     o.ready = true;
 }
 
-template <class P, class G>
-void launch(bool small, const StepArgs& a, unsigned grid, cudaStream_t stream) {
-    if (small) adamw_kernel<P, G, true><<<grid, kThreads, 0, stream>>>(a);
-    else adamw_kernel<P, G, false><<<grid, kThreads, 0, stream>>>(a);
+template <class P, class G, int GRADS>
+void launch(bool small, const StepSettings& settings, const void* const* grads, size_t count, unsigned grid,
+            cudaStream_t stream) {
+    StepArgs<GRADS> a;
+    static_cast<StepSettings&>(a) = settings;
+    std::fill(std::copy_n(grads, count, a.grads), a.grads + GRADS, nullptr);
+    if (small) adamw_kernel<P, G, true, GRADS><<<grid, kThreads, 0, stream>>>(a);
+    else adamw_kernel<P, G, false, GRADS><<<grid, kThreads, 0, stream>>>(a);
     check(cudaGetLastError(), "optimizer launch");
 }
 
@@ -464,7 +473,7 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         std::lock_guard<std::mutex> lock(o.mutex);
         check(cudaSetDevice(o.device), "cudaSetDevice");
         upload(o, static_cast<cudaStream_t>(stream));
-        StepArgs a;
+        StepSettings a;
         const Tile* tiles = static_cast<const Tile*>(o.table);
         const int sms = sm_count(o.device);
         a.lr = (float)lr;
@@ -484,11 +493,14 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
             a.first_tensor = (int32_t)i;
             a.tile_count = (int32_t)count;
             a.tiles = tiles + o.tile_begin[i];
-            std::copy(grads + i, grads + end, a.grads);
+            const unsigned grid = (unsigned)std::min<int64_t>(count, 3 * sms);
+            cudaStream_t s = static_cast<cudaStream_t>(stream);
             by_type(o.dtype, [&](auto p) {
                 by_type(grad_dtype, [&](auto g) {
-                    launch<decltype(p), decltype(g)>(o.state_bits == 8, a, (unsigned)std::min<int64_t>(count, 3 * sms),
-                                                     static_cast<cudaStream_t>(stream));
+                    using P = decltype(p);
+                    using G = decltype(g);
+                    if (end - i <= kFewGrads) launch<P, G, kFewGrads>(o.state_bits == 8, a, grads + i, end - i, grid, s);
+                    else launch<P, G, kGrads>(o.state_bits == 8, a, grads + i, end - i, grid, s);
                 });
             });
         }

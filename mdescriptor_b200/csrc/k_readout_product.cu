@@ -592,10 +592,13 @@ CUtensorMap code_map(const void* base, int64_t rows, int64_t k, int64_t stride, 
     return tile_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k, stride, box_rows);
 }
 
-template <class K, class... Args>
-void launch(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t bytes, cudaStream_t stream,
+// KERNEL is a template argument, so that each kernel has its own record of the
+// devices where its shared memory limit is raised.
+template <auto KERNEL, class... Args>
+void launch(unsigned grid, unsigned cluster, unsigned threads, size_t bytes, int device, cudaStream_t stream,
             const Args&... args) {
-    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), "product shared memory");
+    static std::atomic<uint64_t> done;
+    allow_shared(KERNEL, (int)bytes, done, device, "product shared memory");
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeClusterDimension;
     attribute.val.clusterDim.x = cluster;
@@ -607,7 +610,7 @@ void launch(K kernel, unsigned grid, unsigned cluster, unsigned threads, size_t 
     config.stream = stream;
     config.attrs = &attribute;
     config.numAttrs = 1;
-    check(cudaLaunchKernelEx(&config, kernel, args...), "product launch");
+    check(cudaLaunchKernelEx(&config, KERNEL, args...), "product launch");
 }
 
 // What a product of this shape runs.
@@ -650,20 +653,20 @@ Shape shape_of(int64_t m, int64_t n, int64_t k, int sms) {
 
 template <int COLS, class OUT>
 void run_few(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
-             cudaStream_t stream) {
+             int device, cudaStream_t stream) {
     const CUtensorMap map_a = code_map(a, p.m, p.k, a_stride, COLS), map_b = code_map(b, p.n, p.k, b_stride, kRows);
-    launch(few_product_kernel<COLS, OUT>, (unsigned)(s.tiles * s.splits), (unsigned)s.splits, kFewThreads,
-           sizeof(FewShared<COLS>) + 1024, stream, map_a, map_b, p);
+    launch<few_product_kernel<COLS, OUT>>((unsigned)(s.tiles * s.splits), (unsigned)s.splits, kFewThreads,
+                                          sizeof(FewShared<COLS>) + 1024, device, stream, map_a, map_b, p);
 }
 
 template <bool TILES, class OUT>
 void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
-               int sms, cudaStream_t stream) {
+               int sms, int device, cudaStream_t stream) {
     const CUtensorMap map_a = code_map(a, p.m, p.k, a_stride, kRows), map_b = code_map(b, p.n, p.k, b_stride, kRows);
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(sms / 2, s.tiles * s.splits);
     const size_t bytes = sizeof(PairShared<TILES>) + 1024;
     if (s.splits > 1) {
-        launch(pair_product_kernel<TILES, float, Store::Partial>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_a, p);
+        launch<pair_product_kernel<TILES, float, Store::Partial>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_a, p);
         const dim3 add((unsigned)((p.n + 255) / 256), (unsigned)((p.m + 3) / 4));
         add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
         check(cudaGetLastError(), "product launch");
@@ -672,26 +675,26 @@ void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
         const CUtensorMap map_out =
             tile_map(sizeof(OUT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(OUT),
                      p.out, p.m, p.n, p.out_stride, 32);
-        launch(pair_product_kernel<TILES, OUT, Store::Tile>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_out, p);
+        launch<pair_product_kernel<TILES, OUT, Store::Tile>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_out, p);
     } else {
-        launch(pair_product_kernel<TILES, OUT, Store::Direct>, grid, 2, kThreads, bytes, stream, map_a, map_b, map_a, p);
+        launch<pair_product_kernel<TILES, OUT, Store::Direct>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_a, p);
     }
 }
 
 template <class OUT>
 void run_product(const void* a, int64_t a_stride, const void* b, int64_t b_stride, const ProductArgs& p, const Shape& s,
-                 int sms, cudaStream_t stream) {
+                 int sms, int device, cudaStream_t stream) {
     if (s.few) {
         switch (s.columns) {
-            case 16: run_few<16, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
-            case 32: run_few<32, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
-            case 64: run_few<64, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
-            default: run_few<128, OUT>(a, a_stride, b, b_stride, p, s, stream); break;
+            case 16: run_few<16, OUT>(a, a_stride, b, b_stride, p, s, device, stream); break;
+            case 32: run_few<32, OUT>(a, a_stride, b, b_stride, p, s, device, stream); break;
+            case 64: run_few<64, OUT>(a, a_stride, b, b_stride, p, s, device, stream); break;
+            default: run_few<128, OUT>(a, a_stride, b, b_stride, p, s, device, stream); break;
         }
     } else if (p.b_tiles) {
-        run_pairs<true, OUT>(a, a_stride, b, b_stride, p, s, sms, stream);
+        run_pairs<true, OUT>(a, a_stride, b, b_stride, p, s, sms, device, stream);
     } else {
-        run_pairs<false, OUT>(a, a_stride, b, b_stride, p, s, sms, stream);
+        run_pairs<false, OUT>(a, a_stride, b, b_stride, p, s, sms, device, stream);
     }
 }
 
@@ -742,8 +745,8 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
         ProductArgs p{m, n, k, a_scales, a_scale_stride, b_scales, b_scale_stride, b_tiles, out, out_stride, accumulate};
         p.splits = shape.splits;
         p.partials = static_cast<float*>(workspace);
-        if (out_dtype == MDSOAP_FLOAT32) run_product<float>(a, a_stride, b, b_stride, p, shape, sms, s);
-        else run_product<__nv_bfloat16>(a, a_stride, b, b_stride, p, shape, sms, s);
+        if (out_dtype == MDSOAP_FLOAT32) run_product<float>(a, a_stride, b, b_stride, p, shape, sms, device, s);
+        else run_product<__nv_bfloat16>(a, a_stride, b, b_stride, p, shape, sms, device, s);
     });
 }
 

@@ -25,6 +25,15 @@ inline int sm_count(int device) {
     return sms;
 }
 
+// Raises a kernel's limit of dynamic shared memory, once on each device.
+template <class K>
+void allow_shared(K kernel, int bytes, std::atomic<uint64_t>& done, int device, const char* what) {
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+    done.fetch_or(bit, std::memory_order_release);
+}
+
 template <class F>
 void by_type(int32_t dtype, F&& body) {
     switch (dtype) {
