@@ -11,6 +11,7 @@
 #include "tcgen05.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace mdsoap;
 using namespace mdsoap::readout;
@@ -117,6 +118,7 @@ struct PairShared {
     int issued;
 };
 
+
 constexpr int kStep = 16;  // columns that leave tensor memory at a time
 
 // acc + part x scale for a pair of columns.  Two scalar fmas: as one packed
@@ -126,6 +128,39 @@ __device__ __forceinline__ uint64_t add_scaled(uint32_t x, uint32_t y, uint64_t 
     tc::split_pair(scale, m0, m1);
     tc::split_pair(acc, a0, a1);
     return tc::pair_of(fmaf(__uint_as_float(x), m0, a0), fmaf(__uint_as_float(y), m1, a1));
+}
+
+// A warp's piece of 32 rows x 128 bytes from (swizzled) shared memory to rows of
+// a matrix, BYTES at a time; `cols` elements of each row exist.
+template <class OUT, int BYTES>
+__device__ __forceinline__ void copy_rows(const uint8_t* from, OUT* out, int64_t stride, int rows, int cols, bool add) {
+    using Word = std::conditional_t<BYTES == 8, uint2, std::conditional_t<BYTES == 4, uint32_t, uint16_t>>;
+    constexpr int kAcross = 128 / BYTES;                       // words of a row
+    constexpr int kLanes = kAcross < 32 ? kAcross : 32;        // lanes on one row
+    const int lane = threadIdx.x & 31, r0 = lane / kLanes;
+#pragma unroll 8
+    for (int i = 0; i < kLanes; ++i) {
+        const int r = i * (32 / kLanes) + r0;
+        if (r >= rows) break;
+#pragma unroll
+        for (int k = 0; k < kAcross / kLanes; ++k) {
+            const int byte = (k * kLanes + lane % kLanes) * BYTES;
+            const Word w = *reinterpret_cast<const Word*>(from + r * 128 + ((byte / 16 ^ (r & 7)) * 16) + byte % 16);
+            const int at = byte / (int)sizeof(OUT);
+            if (at >= cols) continue;
+            Word* to = reinterpret_cast<Word*>(out + r * stride + at);
+            if (add) {
+                Word sum = *to;
+                OUT* t = reinterpret_cast<OUT*>(&sum);
+                const OUT* v = reinterpret_cast<const OUT*>(&w);
+#pragma unroll
+                for (int j = 0; j < BYTES / (int)sizeof(OUT); ++j) t[j] = from_float<OUT>(to_float(t[j]) + to_float(v[j]));
+                *to = sum;
+            } else {
+                *to = w;
+            }
+        }
+    }
 }
 
 template <bool TILES, class OUT, Store STORE>
@@ -156,6 +191,10 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
         s.gave_up = 0;
         s.issued = 0;
         bulk::barrier_init_fence();
+    }
+    if (threadIdx.x == kPromote * 32) {
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_b);
     }
     if (warp == kPromote + 1) tc::alloc<2>(&s.tensor_memory, 512);
     tc::fence_before();
@@ -299,52 +338,67 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                 }
             }
             if (*gave_up) break;
-            if constexpr (STORE == Store::Partial) {
+            if constexpr (STORE == Store::Partial && !TILES) {
+                // straight out of the registers: through the copy engine, as below, a part of few blocks ends 4 us
+                // earlier, but this form's loop, short of registers, loses more (1024 x 2100 x 65 537: 281 -> 329 us)
                 float* out = p.partials + ((int64_t)item * kPairTile + rank * kRows + quarter * 32 + lane) * kPairTile + half * kMine;
 #pragma unroll
                 for (int i = 0; i < kMine / 2; i += 2)
                     *reinterpret_cast<ulonglong2*>(out + 2 * i) = make_ulonglong2(acc[i], acc[i + 1]);
-            } else if constexpr (STORE == Store::Tile) {
-                // 128 bytes of each of the warp's rows at a time: 16-byte pieces in the swizzled order the
-                // copy engine expects (piece ^ row % 8), so that neither side meets bank conflicts
-                constexpr int kWide = 128 / (int)sizeof(OUT);
-                uint8_t* mine_out = s.out[warp] + lane * 128;
+            } else {
+                // 128 bytes of each of the warp's rows at a time, through shared memory: 16-byte pieces in the
+                // swizzled order the copy engine expects (piece ^ row % 8), so that no side meets bank conflicts
+                constexpr int kWide = 128 / (int)sizeof(OUT), kEach = 16 / (int)sizeof(OUT);
+                uint8_t* const piece_row = s.out[warp] + lane * 128;
+                const int row0 = m0 + quarter * 32;
 #pragma unroll
                 for (int c = 0; c < kMine; c += kWide) {
-                    if (lane == 0) tc::wait_store_reads();
+                    if (STORE != Store::Direct && lane == 0) tc::wait_store_reads();
                     __syncwarp();
 #pragma unroll
                     for (int piece = 0; piece < 8; ++piece) {
-                        constexpr int kEach = 16 / (int)sizeof(OUT);
                         float f[kEach];
 #pragma unroll
                         for (int i = 0; i < kEach; i += 2)
                             tc::split_pair(acc[(c + piece * kEach + i) / 2], f[i], f[i + 1]);
                         uint4 q;
-                        OUT* t = reinterpret_cast<OUT*>(&q);
-#pragma unroll
-                        for (int i = 0; i < kEach; ++i) t[i] = from_float<OUT>(f[i]);
-                        *reinterpret_cast<uint4*>(mine_out + ((piece ^ (lane & 7)) * 16)) = q;
+                        if constexpr (sizeof(OUT) == 4)
+                            q = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                           __float_as_uint(f[3]));
+                        else
+                            q = make_uint4(pack2<OUT>(f[0], f[1]), pack2<OUT>(f[2], f[3]), pack2<OUT>(f[4 % kEach], f[5 % kEach]),
+                                           pack2<OUT>(f[6 % kEach], f[7 % kEach]));
+                        *reinterpret_cast<uint4*>(piece_row + ((piece ^ (lane & 7)) * 16)) = q;
                     }
-                    bulk::proxy_fence();
-                    __syncwarp();
-                    if (lane == 0 && m0 + quarter * 32 < p.m && col + c < p.n)
-                        tc::store_tile(&map_out, col + c, m0 + quarter * 32, s.out[warp]);
-                }
-            } else {
-                if (row < p.m) {
-                    OUT* out = static_cast<OUT*>(p.out) + (int64_t)row * p.out_stride + col;
-#pragma unroll
-                    for (int c = 0; c < kMine; c += 32) {
-                        float f[32];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) tc::split_pair(acc[c / 2 + i], f[2 * i], f[2 * i + 1]);
-                        store_row(out + c, p.n - col - c, f, p.accumulate);
+                    if constexpr (STORE == Store::Tile) {
+                        bulk::proxy_fence();
+                        __syncwarp();
+                        if (lane == 0 && row0 < p.m && col + c < p.n)
+                            tc::store_tile(&map_out, col + c, row0, s.out[warp]);
+                    } else if constexpr (STORE == Store::Partial) {
+                        bulk::proxy_fence();
+                        __syncwarp();
+                        if (lane == 0)
+                            tc::store_tile(&map_out, half * kMine + c, item * kPairTile + rank * kRows + quarter * 32,
+                                           s.out[warp]);
+                    } else {
+                        // rows that the copy engine cannot write, or that are added to: words as wide as the
+                        // rows' alignment allows, neighbouring lanes on neighbouring words
+                        __syncwarp();
+                        OUT* const out = static_cast<OUT*>(p.out) + (int64_t)row0 * p.out_stride + col + c;
+                        const int rows = min(32, (int)p.m - row0), cols = (int)p.n - col - c;
+                        const uintptr_t mixed = reinterpret_cast<uintptr_t>(out) |
+                                                (uintptr_t)(p.out_stride * (int64_t)sizeof(OUT)) |
+                                                (uintptr_t)(min(cols, kWide) * (int)sizeof(OUT));
+                        if (cols <= 0) continue;
+                        if (mixed % 8 == 0) copy_rows<OUT, 8>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
+                        else if (mixed % 4 == 0) copy_rows<OUT, 4>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
+                        else copy_rows<OUT, sizeof(OUT)>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
                     }
                 }
             }
         }
-        if (STORE == Store::Tile && lane == 0) tc::wait_stores();
+        if (STORE != Store::Direct && lane == 0) tc::wait_stores();
     }
 
     __syncthreads();
@@ -429,6 +483,10 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
         s.gave_up = 0;
         s.issued = 0;
         bulk::barrier_init_fence();
+    }
+    if (threadIdx.x == 4 * 32) {
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_b);
     }
     if (warp == 5) tc::alloc<1>(&s.tensor_memory, kColumns);
     tc::fence_before();
@@ -526,12 +584,26 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
                 }
             }
         }
+        if (parts == 1) {
+            OUT* q = static_cast<OUT*>(p.out) + n;
+            if (n < p.n && !*gave_up) {
 #pragma unroll
-        for (int i = 0; i < COLS / 2; ++i) {
-            float x, y;
-            tc::split_pair(acc[i], x, y);
-            s.sum[2 * i][threadIdx.x] = x;
-            s.sum[2 * i + 1][threadIdx.x] = y;
+                for (int i = 0; i < COLS / 2; ++i) {
+                    float f[2];
+                    tc::split_pair(acc[i], f[0], f[1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j, q += p.out_stride)
+                        if (2 * i + j < (int)p.m) *q = from_float<OUT>(p.accumulate ? to_float(*q) + f[j] : f[j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < COLS / 2; ++i) {
+                float x, y;
+                tc::split_pair(acc[i], x, y);
+                s.sum[2 * i][threadIdx.x] = x;
+                s.sum[2 * i + 1][threadIdx.x] = y;
+            }
         }
     }
 
@@ -542,13 +614,28 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
     }
     tc::cluster_sync();
     const int64_t n = n0 + threadIdx.x;
-    if (threadIdx.x < kRows && n < p.n && !*gave_up) {
-        for (int64_t j = rank; j < p.m; j += parts) {
-            float sum = 0.0f;
-#pragma unroll 8
-            for (int r = 0; r < parts; ++r) sum += tc::load_shared_at(tc::map_shared(&s.sum[j][threadIdx.x], r));
-            OUT* out = static_cast<OUT*>(p.out) + j * p.out_stride + n;
-            *out = from_float<OUT>(p.accumulate ? to_float(*out) + sum : sum);
+    if (parts > 1 && threadIdx.x < kRows && n < p.n && !*gave_up) {
+        OUT* const out = static_cast<OUT*>(p.out) + n;
+        constexpr int kTogether = 8;  // rows whose sums are read at the same time
+        for (int j0 = rank; j0 < (int)p.m; j0 += kTogether * parts) {
+            float sum[kTogether];
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) sum[i] = 0.0f;
+            for (int r = 0; r < parts; ++r) {
+#pragma unroll
+                for (int i = 0; i < kTogether; ++i) {
+                    const int j = min(j0 + i * parts, COLS - 1);
+                    sum[i] += tc::load_shared_at(tc::map_shared(&s.sum[j][threadIdx.x], r));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) {
+                const int j = j0 + i * parts;
+                if (j < (int)p.m) {
+                    OUT* q = out + j * p.out_stride;
+                    *q = from_float<OUT>(p.accumulate ? to_float(*q) + sum[i] : sum[i]);
+                }
+            }
         }
     }
     tc::cluster_sync();  // the others may still read this CTA's sums
@@ -666,7 +753,9 @@ void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
     const unsigned grid = 2 * (unsigned)std::min<int64_t>(sms / 2, s.tiles * s.splits);
     const size_t bytes = sizeof(PairShared<TILES>) + 1024;
     if (s.splits > 1) {
-        launch<pair_product_kernel<TILES, float, Store::Partial>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_a, p);
+        const CUtensorMap map_parts = tile_map(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.partials, s.tiles * s.splits * kPairTile,
+                                               kPairTile, kPairTile, 32);
+        launch<pair_product_kernel<TILES, float, Store::Partial>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_parts, p);
         const dim3 add((unsigned)((p.n + 255) / 256), (unsigned)((p.m + 3) / 4));
         add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
         check(cudaGetLastError(), "product launch");

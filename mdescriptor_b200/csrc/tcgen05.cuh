@@ -167,6 +167,12 @@ __device__ __forceinline__ void load32(uint32_t address, uint32_t (&r)[32]) {
         : "memory");
 }
 __device__ __forceinline__ void load(uint32_t address, uint32_t (&r)[32]) { load32(address, r); }
+__device__ __forceinline__ void load(uint32_t address, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(address)
+                 : "memory");
+}
 __device__ __forceinline__ void load(uint32_t address, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
