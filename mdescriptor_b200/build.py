@@ -7,9 +7,11 @@
   batches (``csrc/synth.c``, gcc + OpenMP; input generation only);
 * ``plugin/_cuda<EXT_SUFFIX>`` -- the pybind11 ``mdescriptor._cuda`` drop-in
   (point ``MDESCRIPTOR_CUDA_PLUGIN_DIR`` at ``plugin/``), linked to
-  ``libmdsoap.so`` through an $ORIGIN rpath.
+  ``libmdsoap.so`` through an $ORIGIN rpath;
+* ``_readout_call<EXT_SUFFIX>`` -- CPython calls of the readout operators'
+  C entry points.
 
-Both are written next to the sources so that they travel with the
+All are written next to the sources so that they travel with the
 repository; nothing is installed into site-packages.
 """
 
@@ -28,6 +30,7 @@ LIB = PACKAGE / "lib" / "libmdsoap.so"
 PLUGIN_DIR = PACKAGE / "plugin"
 OBJ_DIR = PACKAGE / "lib" / "obj"
 SYNTH = PACKAGE / "lib" / "libmdsynth.so"
+READOUT_CALL = PACKAGE / f"_readout_call{sysconfig.get_config_var('EXT_SUFFIX')}"
 PLUGIN = PLUGIN_DIR / f"_cuda{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 NVCC_FLAGS = [
@@ -95,6 +98,14 @@ def build_plugin(force: bool = False) -> Path:
     return PLUGIN
 
 
+def build_readout_call(force: bool = False) -> Path:
+    source = CSRC / "readout_call.cpp"
+    if force or _stale(READOUT_CALL, [source, INCLUDE / "mdsoap.h"]):
+        _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+              f"-I{sysconfig.get_paths()['include']}", str(source), "-o", str(READOUT_CALL)])
+    return READOUT_CALL
+
+
 def build_synth(force: bool = False) -> Path:
     """The seeded batch generator for the large benchmark configs (host C)."""
     source = CSRC / "synth.c"
@@ -107,6 +118,7 @@ def build_synth(force: bool = False) -> Path:
 def build_all(force: bool = False, verbose: bool = False) -> None:
     build_library(force, verbose)
     build_plugin(force)
+    build_readout_call(force)
     build_synth(force)
 
 

@@ -33,6 +33,15 @@ import torch
 from . import _lib
 from ._lib import AdamWParams, lib, raise_for
 
+try:
+    from . import _readout_call as _call
+except ImportError as error:  # no second way: a missing build is an error, as with the library
+    raise ImportError("readout calls not built; run `python -m mdescriptor_b200.build`") from error
+
+_call.bind(*(ctypes.cast(f, ctypes.c_void_p).value
+             for f in (lib.mdsoap_rms_norm, lib.mdsoap_rms_norm_backward, lib.mdsoap_quantize, lib.mdsoap_matmul,
+                       lib.mdsoap_adamw_step)))
+
 BLOCK = 128
 
 _DTYPES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
@@ -155,9 +164,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
         out, out_stride, scale_stride = _empty_blocks(rows, width, rows, device)
         out_ptr, scales_ptr = out.values.data_ptr(), out.scales.data_ptr()
     if rows and width:
-        raise_for(lib.mdsoap_rms_norm(
+        status = _call.rms_norm(
             x.data_ptr(), rows, width, stride, residual_ptr, residual_stride, dtype, weight_ptr, eps, sum_ptr, width,
-            rstd.data_ptr(), out_ptr, out_stride, scales_ptr, scale_stride, index, _stream(index)))
+            rstd.data_ptr(), out_ptr, out_stride, scales_ptr, scale_stride, index, _stream(index))
+        if status:
+            raise_for(status)
     return Norm(out, total, rstd)
 
 
@@ -187,7 +198,7 @@ def rms_norm_backward(dy: torch.Tensor, sum: torch.Tensor, rstd: torch.Tensor, w
     dx = torch.empty((rows, width), dtype=sum.dtype, device=sum.device)
     dweight = torch.empty(width, dtype=torch.float32, device=sum.device)
     workspace = torch.empty(bytes_, dtype=torch.uint8, device=sum.device)
-    raise_for(lib.mdsoap_rms_norm_backward(
+    raise_for(_call.rms_norm_backward(
         dy.data_ptr(), rows, width, dy_stride, sum.data_ptr(), stride, rstd_ptr, weight_ptr,
         None if dsum is None else dsum.data_ptr(), dsum_stride, dtype, dx.data_ptr(), width, dweight.data_ptr(),
         workspace.data_ptr(), bytes_, device, _stream(device)))
@@ -221,27 +232,29 @@ def quantize(x: torch.Tensor, layout: str = "rows", row_factor: torch.Tensor | N
                                                            device)
         codes_t, scales_t = by_columns.values.data_ptr(), by_columns.scales.data_ptr()
     if rows and width:
-        raise_for(lib.mdsoap_quantize(x.data_ptr(), rows, width, stride, dtype, row_ptr, col_ptr, tiles, codes, pitch,
-                                      scales, scale_pitch, codes_t, pitch_t, scales_t, scale_pitch_t, index,
-                                      _stream(index)))
+        status = _call.quantize(x.data_ptr(), rows, width, stride, dtype, row_ptr, col_ptr, tiles, codes, pitch, scales,
+                                scale_pitch, codes_t, pitch_t, scales_t, scale_pitch_t, index, _stream(index))
+        if status:
+            raise_for(status)
     return Quantized(by_rows, by_columns)
 
 
-def _blocks(b: Blocks, name: str, tiles: bool) -> tuple[int, int, int, int, bool]:
-    """(rows, width, pitch, scale pitch, scales of tiles) of checked blocks."""
+def _blocks(b: Blocks, name: str, tiles: bool) -> tuple[int, int, int, int, int, int, bool]:
+    """(rows, width, address, pitch, scales' address, their pitch, scales of tiles) of checked blocks."""
     values, scales = b
     rows, width, stride = _matrix(values, f"{name}.values")
+    scale_rows, blocks, scale_stride = _matrix(scales, f"{name}.scales")
     if values.dtype != _CODES:
         raise ValueError(f"{name}.values must be float8_e4m3fn, got {values.dtype}")
-    scale_rows, blocks, scale_stride = _matrix(scales, f"{name}.scales")
     if scales.dtype != torch.float32 or scales.get_device() != values.get_device():
         raise ValueError(f"{name}.scales must be float32 on {values.device}")
     by_rows = scale_rows == rows
-    if blocks != (width + BLOCK - 1) // BLOCK or not (by_rows or (tiles and scale_rows == (rows + BLOCK - 1) // BLOCK)):
+    if blocks != (width + 127) // 128 or not (by_rows or (tiles and scale_rows == (rows + 127) // 128)):
         raise ValueError(f"{name}.scales has shape {tuple(scales.shape)}, which fits no blocks of {tuple(values.shape)}")
-    if rows and width and (stride % 16 or values.data_ptr() % 16):
+    address = values.data_ptr()
+    if (stride % 16 or address % 16) and rows and width:
         raise ValueError(f"{name}.values must start on 16 bytes and have a row pitch that is a multiple of 16")
-    return rows, width, stride, scale_stride, not by_rows
+    return rows, width, address, stride, scales.data_ptr(), scale_stride, not by_rows
 
 
 @lru_cache(maxsize=4096)
@@ -258,8 +271,8 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
     ``b`` may carry scales of tiles (weights) or of its rows (the weight's
     gradient).  ``dtype`` "bfloat16" or "float32"; ``out`` takes the result, and
     with ``accumulate`` (float32) has it added."""
-    m, k, a_stride, a_scale_stride, _ = _blocks(a, "a", False)
-    n, k_b, b_stride, b_scale_stride, tiles = _blocks(b, "b", True)
+    m, k, a_ptr, a_stride, a_scale_ptr, a_scale_stride, _ = _blocks(a, "a", False)
+    n, k_b, b_ptr, b_stride, b_scale_ptr, b_scale_stride, tiles = _blocks(b, "b", True)
     if k != k_b:
         raise ValueError(f"a and b must have the same width, got {k} and {k_b}")
     device, index = a.values.device, a.values.get_device()
@@ -282,10 +295,11 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
             raise ValueError("accumulate needs a float32 out")
     bytes_ = _matmul_bytes(m, n, k, tiles, index)
     workspace = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
-    raise_for(lib.mdsoap_matmul(
-        a.values.data_ptr(), m, a_stride, a.scales.data_ptr(), a_scale_stride, b.values.data_ptr(), n, b_stride,
-        b.scales.data_ptr(), b_scale_stride, tiles, k, _DTYPES[kind], accumulate, out.data_ptr(), out_stride,
-        None if workspace is None else workspace.data_ptr(), bytes_, index, _stream(index)))
+    status = _call.matmul(
+        a_ptr, m, a_stride, a_scale_ptr, a_scale_stride, b_ptr, n, b_stride, b_scale_ptr, b_scale_stride, tiles, k, _DTYPES[kind], accumulate, out.data_ptr(), out_stride,
+        None if workspace is None else workspace.data_ptr(), bytes_, index, _stream(index))
+    if status:
+        raise_for(status)
     return out
 
 
@@ -368,8 +382,8 @@ class AdamW:
             raise ValueError(f"grads must be contiguous tensors of one type on {self.device}")
         step = self.state["step"] + 1
         pointers = array("Q", map(torch.Tensor.data_ptr, grads))
-        raise_for(lib.mdsoap_adamw_step(
-            self._optimizer, pointers.buffer_info()[0], _dtype(grads[0], "grads"), step, self.lr if lr is None else lr,
+        raise_for(_call.adamw_step(
+            self._optimizer.value, pointers.buffer_info()[0], _dtype(grads[0], "grads"), step, self.lr if lr is None else lr,
             self.betas[0], self.betas[1], self.eps, grad_scale, _stream(self.device.index)))
         self.state["step"] = step
 
