@@ -133,11 +133,6 @@ __device__ __forceinline__ void decode(uint32_t codes, float scale, float (&f)[4
     }
 }
 
-__device__ __forceinline__ float reciprocal(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ float square_root(float x) {
     float r;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -155,7 +150,7 @@ __device__ __forceinline__ float square_root(float x) {
 template <bool FLOOR>
 __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (&u20)[4], float& scale) {
     const float top = warp_larger(larger(larger(x[0], x[1], x[2]), x[3]));
-    scale = top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop);
+    scale = scale_of(top);
     const float inverse = reciprocal(scale);
     float a[4], least = kTop;
 #pragma unroll

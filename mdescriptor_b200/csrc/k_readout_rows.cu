@@ -77,7 +77,7 @@ struct RowPass {
             }
         }
         if constexpr (MODE != Rows::NormWide) {
-            float4 z = s, rest = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float4 z = s;
             if (MODE == Rows::Norm8 || a.col_factor) {
                 float4 w;
                 if constexpr (FULL) {
@@ -88,15 +88,13 @@ struct RowPass {
                     w = make_float4(f[0], f[1], f[2], f[3]);
                 }
                 z = make_float4(s.x * w.x, s.y * w.y, s.z * w.z, s.w * w.w);
-                rest = make_float4(fmaf(s.x, w.x, -z.x), fmaf(s.y, w.y, -z.y), fmaf(s.z, w.z, -z.z),
-                                   fmaf(s.w, w.w, -z.w));
             }
             const float most = warp_larger(larger(larger(z.x, z.y, z.z), z.w));
             const Factor factor(most);
             if (FULL || col < width) {  // the pitch covers a quad's padding
                 if (lane == 0) top[col / kBlock] = most;
                 *reinterpret_cast<uint32_t*>(codes + col) =
-                    codes4(factor(z.x, rest.x), factor(z.y, rest.y), factor(z.z, rest.z), factor(z.w, rest.w));
+                    codes4(factor(z.x), factor(z.y), factor(z.z), factor(z.w));
             }
         }
     }
@@ -606,8 +604,11 @@ struct TileArgs {
 // reads along a column are free of bank conflicts.
 // TILES: one scale for the whole tile, in both directions.
 // Bound by HBM: every element once in, one byte out a direction.
+// Two CTAs an SM with both directions of 16-bit elements (37 us for 32 771 x 1024,
+// 45 with three, whose 80 registers do not hold the passes), else three, or two
+// for the 64 registers that float32 quads fill.
 template <class T, bool ROWS, bool TILES>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const __grid_constant__ TileArgs<T> a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 || (ROWS && !TILES) ? 2 : 3) void tile_kernel(const __grid_constant__ TileArgs<T> a) {
     using Word = typename Quad<T>::Word;
     __shared__ __align__(16) uint8_t s_codes[128 * 128];
     __shared__ __align__(16) float s_top[8][128];
@@ -652,6 +653,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
         col_top = make_float4(larger(col_top.x, x.x, y.x), larger(col_top.y, x.y, y.y), larger(col_top.z, x.z, y.z),
                               larger(col_top.w, x.w, y.w));
     }
+    // Between the passes over the quads: they are unpacked again each time, 64 floats would not fit the registers.
+    const auto forget = [&] {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("" : "+r"(raw[i].x), "+r"(raw[i].y));
+    };
+    forget();
     if constexpr (ROWS && !TILES) {
         // The rows' maxima first; lane i then works out row i's factor for all lanes.
         float mine = 0.0f;
@@ -663,26 +670,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
             if (lane == i) mine = top;
         }
         const Factor own(mine);
+        forget();
         const int64_t own_row = tile_row + row0 + lane;
         if (lane < 16 && own_row < rows)
             a.scales[own_row * a.scale_stride + blockIdx.x] = scale_of(mine) * (row_factor ? s_factor[row0 + lane] : 1.0f);
         uint8_t* out = a.codes + (tile_row + row0) * a.code_stride + col;
+        const int here = col < width ? (int)min((int64_t)16, rows - tile_row - row0) : 0;  // rows to write
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float4 x = unpack4<T>(raw[i]);
             Factor factor(0.0f);
-            factor.hi = __shfl_sync(0xffffffffu, own.hi, i);
-            factor.lo = __shfl_sync(0xffffffffu, own.lo, i);
+            factor.inverse = __shfl_sync(0xffffffffu, own.inverse, i);
+            factor.scale = __shfl_sync(0xffffffffu, own.scale, i);
             uint32_t q;
             if (col_factor) {
-                const float4 z = make_float4(x.x * g[0], x.y * g[1], x.z * g[2], x.w * g[3]);
-                q = codes4(factor(z.x, fmaf(x.x, g[0], -z.x)), factor(z.y, fmaf(x.y, g[1], -z.y)),
-                           factor(z.z, fmaf(x.z, g[2], -z.z)), factor(z.w, fmaf(x.w, g[3], -z.w)));
+                q = codes4(factor(x.x * g[0]), factor(x.y * g[1]), factor(x.z * g[2]), factor(x.w * g[3]));
             } else {
                 q = codes4(factor(x.x), factor(x.y), factor(x.z), factor(x.w));
             }
-            if (tile_row + row0 + i < rows && col < width) *reinterpret_cast<uint32_t*>(out + i * a.code_stride) = q;
+            if (i < here) *reinterpret_cast<uint32_t*>(out) = q;
+            out += a.code_stride;
+            asm volatile("" : "+l"(out));  // one address on its way through the rows, not sixteen
         }
+        forget();
     }
 
     if constexpr (TILES) {
@@ -737,14 +747,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void tile_kernel(const
             make_uint4(piece[0], piece[1], piece[2], piece[3]);
     }
     if constexpr (TILES && ROWS) {
+        forget();
         const Factor factor(col_top.x);
+        uint8_t* out = a.codes + (tile_row + row0) * a.code_stride + col;
+        const int here = col < width ? (int)min((int64_t)16, rows - tile_row - row0) : 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const int64_t row = tile_row + row0 + i;
             const float4 x = unpack4<T>(raw[i]);
-            if (row < rows && col < width)
-                *reinterpret_cast<uint32_t*>(a.codes + row * a.code_stride + col) =
-                    codes4(factor(x.x), factor(x.y), factor(x.z), factor(x.w));
+            if (i < here)
+                *reinterpret_cast<uint32_t*>(out) = codes4(factor(x.x), factor(x.y), factor(x.z), factor(x.w));
+            out += a.code_stride;
+            asm volatile("" : "+l"(out));
         }
     }
     __syncthreads();

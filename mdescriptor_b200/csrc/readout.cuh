@@ -357,39 +357,44 @@ __device__ __forceinline__ float warp_larger(float most) {
     return r;
 }
 
-// 448 / top as a sum hi + lo, good to about 2^-40, so that fma(z, hi, z * lo) is
-// 448 z / top rounded once: an entry that lies on a tie between two codes is
-// seen as one.  Zero for a block that is stored as zeros.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// A block's scale; the constant is the rounded reciprocal of 448.
+__device__ __forceinline__ float scale_of(float top) { return top < kTiny ? 0.0f : __fmul_rn(top, 1.0f / kTop); }
+
+// z / scale for the entries of a block with the maximum `top`: the quick
+// reciprocal's product with one correction by its exact remainder, which leaves
+// the correctly rounded quotient but for about one entry in a million.  Zero in
+// a block that is stored as zeros, and for the finite entries beside an
+// infinite one.
 struct Factor {
-    float hi, lo;
+    float inverse, scale;
     __device__ __forceinline__ explicit Factor(float top) {
-        // any close value does for hi, lo holds the rest; 2^-10 keeps the quick division's divisor below 2^126
-        hi = __fdividef(kTop * 0x1p-10f, top * 0x1p-10f);
-        lo = fmaf(-hi, top, kTop) * (hi * (1.0f / kTop));
-        if (top == INFINITY) lo = 0.0f;
-        if (top < kTiny) hi = lo = 0.0f;
+        scale = scale_of(top);
+        inverse = reciprocal(scale);
+        if (top < kTiny || top == INFINITY) inverse = scale = 0.0f;
     }
-    __device__ __forceinline__ float operator()(float z) const { return fmaf(z, hi, z * lo); }
-    // the same for two exact products x f, in packed arithmetic
+    __device__ __forceinline__ float operator()(float z) const {
+        const float q = z * inverse;
+        return fmaf(fmaf(-q, scale, z), inverse, q);
+    }
+    // the same for x f and y f' (the factors as a pair), in packed arithmetic
     __device__ __forceinline__ void pair(float x, float y, uint64_t f, float& q, float& r) const {
-        asm("{\n\t.reg .b64 x, z, n, e, h, l, q;\n\t"
-            "mov.b64 x, {%2, %3};\n\tmov.b64 h, {%5, %5};\n\tmov.b64 l, {%6, %6};\n\t"
-            "mov.b64 n, {%7, %7};\n\t"
-            "mul.rn.f32x2 z, x, %4;\n\t"
-            "mul.rn.f32x2 n, z, n;\n\t"
-            "fma.rn.f32x2 e, x, %4, n;\n\t"
-            "mul.rn.f32x2 e, e, h;\n\t"
-            "fma.rn.f32x2 e, z, l, e;\n\t"
-            "fma.rn.f32x2 q, z, h, e;\n\t"
+        asm("{\n\t.reg .b64 z, n, i, q;\n\t"
+            "mov.b64 z, {%2, %3};\n\tmov.b64 i, {%5, %5};\n\tmov.b64 n, {%6, %6};\n\t"
+            "mul.rn.f32x2 z, z, %4;\n\t"
+            "mul.rn.f32x2 q, z, i;\n\t"
+            "fma.rn.f32x2 z, q, n, z;\n\t"
+            "fma.rn.f32x2 q, z, i, q;\n\t"
             "mov.b64 {%0, %1}, q;\n\t}"
             : "=f"(q), "=f"(r)
-            : "f"(x), "f"(y), "l"(f), "f"(hi), "f"(lo), "f"(-1.0f));
+            : "f"(x), "f"(y), "l"(f), "f"(inverse), "f"(-scale));
     }
-    // the same for z + rest, the exact product of two floats
-    __device__ __forceinline__ float operator()(float z, float rest) const { return fmaf(z, hi, fmaf(z, lo, rest * hi)); }
 };
-
-__device__ __forceinline__ float scale_of(float top) { return top < kTiny ? 0.0f : __fdiv_rn(top, kTop); }
 
 // Two e4m3 codes, `a` in the low byte.
 __device__ __forceinline__ uint32_t codes2(float a, float b) {
