@@ -403,8 +403,8 @@ int mdsoap_local_compute(const mdsoap_local_params* params, const mdsoap_batch* 
  * of 16 (the bytes between the width and the next multiple of 16 may be
  * written), and one float32 scale for each block of 128 neighbouring entries
  * of a row: scales[row][block], pitch at least ceil(width / 128).  A block z
- * with A = max |z| holds the codes e4m3(448 z / A) (to nearest, ties to even)
- * and the scale A / 448; a block with A < 2^-100 zero codes and scale 0.  A
+ * with A = max |z| holds the scale A / 448 and the codes e4m3(z / scale), to
+ * nearest, ties to even; a block with A < 2^-100 zero codes and scale 0.  A
  * NaN makes its block NaN; an infinite A leaves zeros for finite entries and
  * NaN for the infinite ones. */
 

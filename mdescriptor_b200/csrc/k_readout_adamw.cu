@@ -194,7 +194,10 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 // to v more than b2 takes away; a positive v keeps at least the smallest code,
 // since a zero under a non-zero m would make a huge step.  A NaN or infinite
 // moment shows in its block's scale.
-// Bound by HBM: p, m, v in and out, g in.
+// Bound by HBM (p, m, v in and out, g in) with states of 32 bits; with 8 bits the
+// arithmetic is as long as the traffic: 64 M elements in 211 tensors, float32 p,
+// bfloat16 g, 207 us a step, 4.4 TB/s, 68 % of issue slots used (365 us with exact
+// divisions and codes by conversion).
 template <class P, class G, bool SMALL>
 struct Update {
     const StepSettings& a;

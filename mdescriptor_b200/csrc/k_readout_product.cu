@@ -94,6 +94,19 @@ __device__ __forceinline__ void store_row(OUT* p, int64_t left, const float (&f)
 // the first CTA issues the matrix instructions, warps 0 to 7 scale and add.
 // Persistent: the pairs take tiles (and parts of K) in turn, columns first, so
 // that the pairs at work share A's rows and B stays in L2.
+//
+// Measured: 131 072 x 4096 x 3696 into bfloat16 2.45 to 2.50 ms, 1.6 PFLOP/s, with
+// the board at its power limit (1.65 GHz at 1000 W); 128 x 128 tiles of one CTA
+// took 3.95 ms.  Two accumulators fill tensor memory, so a block's matrix
+// instructions (512 clocks) wait until its accumulator of two blocks ago has been
+// read: commit, wake, read and arrival take another 1000 to 1500 clocks for every
+// two blocks.  Without the multiplications the same loop takes 2.0 ms, without
+// reading tensor memory 1.9, the copies alone 1.4 (10.8 TB/s out of L2).  Four
+// accumulators of half the columns took 2.7 ms (each instruction reads A again),
+// sixteen warps with half the columns each 2.8 (registers).
+// Scales of B's rows instead of tiles cost a multiplication and a read of shared
+// memory more for every product: 1024 x 2100 x 65 537 into float32 281 us, 1.0
+// PFLOP/s.
 
 constexpr int kPairTile = 256;
 constexpr int kPromote = 8;                    // warps that scale and add the partial products
@@ -439,6 +452,9 @@ __global__ __launch_bounds__(256) void add_parts_kernel(const __grid_constant__ 
 // to COLS) as the columns, so each 16 KB of B travel beside COLS / 8 KB of A.
 // The CTAs of a cluster share K, each adds up its part, and they join their sums
 // through each other's shared memory in the cluster's order.
+// One row x 1024 x 3696: 6.4 us back to back on the device (9.3 us a call from
+// Python), of which its 3.8 MB take 0.6 us: launch, cluster barriers and the first
+// copies' latency are the rest.
 
 constexpr int kFewThreads = 6 * 32;  // four warps that scale and add, one for the copies, one for the instructions
 

@@ -2,7 +2,7 @@
 // at any alignment, e4m3 blocks of 128, element types.
 //
 // A block of 128 entries z with A = max |z| is stored as the codes
-// e4m3(448 z / A) and the float32 scale A / 448; a block with A < 2^-100 as
+// e4m3(z / scale) with the float32 scale A / 448; a block with A < 2^-100 as
 // zero codes with scale 0.  A NaN in a block makes A and so the whole block
 // NaN; an infinite A leaves zeros for the finite entries and NaN for the rest.
 #pragma once
