@@ -144,36 +144,49 @@ __device__ __forceinline__ uint64_t add_scaled(uint32_t x, uint32_t y, uint64_t 
 }
 
 // A warp's piece of 32 rows x 128 bytes from (swizzled) shared memory to rows of
-// a matrix, BYTES at a time; `cols` elements of each row exist.
-template <class OUT, int BYTES>
+// a matrix, BYTES at a time; `rows` rows and `cols` elements of each exist.
+// WHOLE: all of them, and nothing is added, so that reads and writes need not wait
+// for one another.
+template <class OUT, int BYTES, bool WHOLE>
 __device__ __forceinline__ void copy_rows(const uint8_t* from, OUT* out, int64_t stride, int rows, int cols, bool add) {
     using Word = std::conditional_t<BYTES == 8, uint2, std::conditional_t<BYTES == 4, uint32_t, uint16_t>>;
     constexpr int kAcross = 128 / BYTES;                       // words of a row
     constexpr int kLanes = kAcross < 32 ? kAcross : 32;        // lanes on one row
-    const int lane = threadIdx.x & 31, r0 = lane / kLanes;
+    constexpr int kRowsAtOnce = 32 / kLanes;
+    const int lane = threadIdx.x & 31;
+    out += lane / kLanes * stride + lane % kLanes * (BYTES / (int)sizeof(OUT));
 #pragma unroll 8
-    for (int i = 0; i < kLanes; ++i) {
-        const int r = i * (32 / kLanes) + r0;
-        if (r >= rows) break;
+    for (int i = 0; i < kLanes; ++i, out += kRowsAtOnce * stride) {
+        const int r = i * kRowsAtOnce + lane / kLanes;
+        if (!WHOLE && r >= rows) break;
 #pragma unroll
         for (int k = 0; k < kAcross / kLanes; ++k) {
             const int byte = (k * kLanes + lane % kLanes) * BYTES;
             const Word w = *reinterpret_cast<const Word*>(from + r * 128 + ((byte / 16 ^ (r & 7)) * 16) + byte % 16);
-            const int at = byte / (int)sizeof(OUT);
-            if (at >= cols) continue;
-            Word* to = reinterpret_cast<Word*>(out + r * stride + at);
-            if (add) {
-                Word sum = *to;
-                OUT* t = reinterpret_cast<OUT*>(&sum);
-                const OUT* v = reinterpret_cast<const OUT*>(&w);
-#pragma unroll
-                for (int j = 0; j < BYTES / (int)sizeof(OUT); ++j) t[j] = from_float<OUT>(to_float(t[j]) + to_float(v[j]));
-                *to = sum;
-            } else {
+            Word* to = reinterpret_cast<Word*>(out + k * kLanes * (BYTES / (int)sizeof(OUT)));
+            if constexpr (WHOLE) {
                 *to = w;
+            } else {
+                if (byte / (int)sizeof(OUT) >= cols) continue;
+                if (add) {
+                    Word sum = *to;
+                    OUT* t = reinterpret_cast<OUT*>(&sum);
+                    const OUT* v = reinterpret_cast<const OUT*>(&w);
+#pragma unroll
+                    for (int j = 0; j < BYTES / (int)sizeof(OUT); ++j) t[j] = from_float<OUT>(to_float(t[j]) + to_float(v[j]));
+                    *to = sum;
+                } else {
+                    *to = w;
+                }
             }
         }
     }
+}
+
+template <class OUT, int BYTES>
+__device__ __forceinline__ void copy_rows(const uint8_t* from, OUT* out, int64_t stride, int rows, int cols, bool add) {
+    if (rows >= 32 && cols >= 128 / (int)sizeof(OUT) && !add) copy_rows<OUT, BYTES, true>(from, out, stride, rows, cols, false);
+    else copy_rows<OUT, BYTES, false>(from, out, stride, rows, cols, add);
 }
 
 template <bool TILES, class OUT, Store STORE>

@@ -63,8 +63,8 @@ struct RowPass {
     uintptr_t x_begin, x_end, r_begin, r_end;
     float total;
 
-    // One block from its words.  FULL: all 128 columns exist, rows and factors are aligned to words.
-    template <bool FULL>
+    // One whole block from its words.  ALIGNED: rows and factors can be read and written in words.
+    template <bool ALIGNED>
     __device__ __forceinline__ void block(int col, const Word& wx, const Word& wr) {
         const int lane = threadIdx.x & 31;
         float4 s = unpack4<T>(wx);
@@ -75,7 +75,7 @@ struct RowPass {
         if constexpr (MODE != Rows::Quantize) {
             total = fmaf(s.x, s.x, fmaf(s.y, s.y, fmaf(s.z, s.z, fmaf(s.w, s.w, total))));
             if (sum) {
-                if constexpr (FULL) *reinterpret_cast<Word*>(sum + col) = pack4<T>(s);
+                if constexpr (ALIGNED) *reinterpret_cast<Word*>(sum + col) = pack4<T>(s);
                 else store_quad(sum, col, width, pack4<T>(s));
             }
         }
@@ -83,7 +83,7 @@ struct RowPass {
             float4 z = s;
             if (MODE == Rows::Norm8 || a.col_factor) {
                 float4 w;
-                if constexpr (FULL) {
+                if constexpr (ALIGNED) {
                     w = __ldg(reinterpret_cast<const float4*>(a.col_factor + col));
                 } else {
                     float f[4];
@@ -94,11 +94,8 @@ struct RowPass {
             }
             const float most = warp_larger(larger(larger(z.x, z.y, z.z), z.w));
             const Factor factor(most);
-            if (FULL || col < width) {  // the pitch covers a quad's padding
-                if (lane == 0) top[col / kBlock] = most;
-                *reinterpret_cast<uint32_t*>(codes + col) =
-                    codes4(factor(z.x), factor(z.y), factor(z.z), factor(z.w));
-            }
+            if (lane == 0) top[col / kBlock] = most;
+            *reinterpret_cast<uint32_t*>(codes + col) = codes4(factor(z.x), factor(z.y), factor(z.z), factor(z.w));
         }
     }
 
@@ -118,6 +115,40 @@ struct RowPass {
         for (int i = 0; i < kAhead; ++i) block<ALIGNED>(col + i * kStep * kBlock, wx[i], wr[i]);
     }
 
+    // One block element by element, a lane every 32nd, each access of the warp a run of neighbouring ones: the last
+    // of a row, and what is left over.
+    __device__ __forceinline__ void scattered(int b) {
+        const int lane = threadIdx.x & 31, col = b * kBlock + lane;
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool live = col + 32 * i < width;
+            s[i] = live ? to_float(x[col + 32 * i]) : 0.0f;
+            if (r && live) s[i] += to_float(r[col + 32 * i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool live = col + 32 * i < width;
+            if constexpr (MODE != Rows::Quantize) {
+                total = fmaf(s[i], s[i], total);
+                if (sum && live) sum[col + 32 * i] = from_float<T>(s[i]);
+            }
+            if (MODE != Rows::NormWide && live && (MODE == Rows::Norm8 || a.col_factor))
+                s[i] *= __ldg(a.col_factor + col + 32 * i);
+        }
+        if constexpr (MODE != Rows::NormWide) {
+            const float most = warp_larger(larger(larger(s[0], s[1], s[2]), s[3]));
+            const Factor factor(most);
+            if (lane == 0) top[b] = most;
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const uint32_t q = codes2(factor(s[i]), factor(s[i + 1]));
+                if (col + 32 * i < width) codes[col + 32 * i] = (uint8_t)q;
+                if (col + 32 * i + 32 < width) codes[col + 32 * i + 32] = (uint8_t)(q >> 8);
+            }
+        }
+    }
+
     // Whether the aligned words around columns [0, columns) of a row lie inside its matrix.
     __device__ __forceinline__ bool inside(const T* row, int columns, uintptr_t begin, uintptr_t end) const {
         const uintptr_t at = reinterpret_cast<uintptr_t>(row), shift = at % sizeof(Word);
@@ -126,21 +157,20 @@ struct RowPass {
 
     // The warp's blocks: kAhead of them under way at a time.
     __device__ __forceinline__ void run(int first) {
-        const int lane = threadIdx.x & 31;
         const int full = width / kBlock;
         int b = first;
         if (quads_aligned(x) && (!r || quads_aligned(r)) && (!sum || quads_aligned(sum)) &&
             reinterpret_cast<uintptr_t>(a.col_factor) % 16 == 0) {
             for (; b + (kAhead - 1) * kStep < full; b += kAhead * kStep) several<true>(b);
+            for (; b < full; b += kStep) {
+                const int col = b * kBlock + (int)(threadIdx.x & 31) * 4;
+                block<true>(col, __ldg(reinterpret_cast<const Word*>(x + col)),
+                            r ? __ldg(reinterpret_cast<const Word*>(r + col)) : Word{});
+            }
         } else if (inside(x, full * kBlock, x_begin, x_end) && (!r || inside(r, full * kBlock, r_begin, r_end))) {
             for (; b + (kAhead - 1) * kStep < full; b += kAhead * kStep) several<false>(b);
         }
-        for (; b * kBlock < width; b += kStep) {
-            const int col = b * kBlock + lane * 4;
-            const Word wx = load_quad(x, col, width, x_begin, x_end);
-            const Word wr = r ? load_quad(r, col, width, r_begin, r_end) : Word{};
-            block<false>(col, wx, wr);
-        }
+        for (; b * kBlock < width; b += kStep) scattered(b);
     }
 };
 
