@@ -120,10 +120,11 @@ enum class Store { Tile, Direct, Partial };
 
 template <bool TILES>
 struct PairShared {
-    static constexpr int kStages = TILES ? 6 : 5;
+    static constexpr int kStages = 5;
+    static constexpr int kOut = TILES ? 2 : 1;  // pieces of a warp's results on their way out at a time
     uint8_t a[kStages][kRows * kTileK];
     uint8_t b[kStages][kRows * kTileK];
-    uint8_t out[kPromote][32 * 128];  // one 128-byte piece of each of a warp's rows on its way out
+    uint8_t out[kOut][kPromote][32 * 128];  // 128-byte pieces of a warp's 32 rows
     float b_scale[TILES ? 1 : 2][4][TILES ? 4 : kPairTile];
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
     uint32_t tensor_memory;
@@ -375,11 +376,12 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                 // 128 bytes of each of the warp's rows at a time, through shared memory: 16-byte pieces in the
                 // swizzled order the copy engine expects (piece ^ row % 8), so that no side meets bank conflicts
                 constexpr int kWide = 128 / (int)sizeof(OUT), kEach = 16 / (int)sizeof(OUT);
-                uint8_t* const piece_row = s.out[warp] + lane * 128;
                 const int row0 = m0 + quarter * 32;
 #pragma unroll
                 for (int c = 0; c < kMine; c += kWide) {
-                    if (STORE != Store::Direct && lane == 0) tc::wait_store_reads();
+                    uint8_t* const piece_out = s.out[c / kWide % S::kOut][warp];
+                    uint8_t* const piece_row = piece_out + lane * 128;
+                    if (STORE != Store::Direct && lane == 0) tc::wait_store_reads<S::kOut - 1>();
                     __syncwarp();
 #pragma unroll
                     for (int piece = 0; piece < 8; ++piece) {
@@ -399,14 +401,18 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                     if constexpr (STORE == Store::Tile) {
                         bulk::proxy_fence();
                         __syncwarp();
-                        if (lane == 0 && row0 < p.m && col + c < p.n)
-                            tc::store_tile(&map_out, col + c, row0, s.out[warp]);
+                        if (lane == 0) {
+                            if (row0 < p.m && col + c < p.n) tc::store_tile(&map_out, col + c, row0, piece_out);
+                            tc::end_stores();  // a group a piece, so that the wait counts pieces
+                        }
                     } else if constexpr (STORE == Store::Partial) {
                         bulk::proxy_fence();
                         __syncwarp();
-                        if (lane == 0)
+                        if (lane == 0) {
                             tc::store_tile(&map_out, half * kMine + c, item * kPairTile + rank * kRows + quarter * 32,
-                                           s.out[warp]);
+                                           piece_out);
+                            tc::end_stores();
+                        }
                     } else {
                         // rows that the copy engine cannot write, or that are added to: words as wide as the
                         // rows' alignment allows, neighbouring lanes on neighbouring words
@@ -417,14 +423,14 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                                                 (uintptr_t)(p.out_stride * (int64_t)sizeof(OUT)) |
                                                 (uintptr_t)(min(cols, kWide) * (int)sizeof(OUT));
                         if (cols <= 0) continue;
-                        if (mixed % 8 == 0) copy_rows<OUT, 8>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
-                        else if (mixed % 4 == 0) copy_rows<OUT, 4>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
-                        else copy_rows<OUT, sizeof(OUT)>(s.out[warp], out, p.out_stride, rows, cols, p.accumulate);
+                        if (mixed % 8 == 0) copy_rows<OUT, 8>(piece_out, out, p.out_stride, rows, cols, p.accumulate);
+                        else if (mixed % 4 == 0) copy_rows<OUT, 4>(piece_out, out, p.out_stride, rows, cols, p.accumulate);
+                        else copy_rows<OUT, sizeof(OUT)>(piece_out, out, p.out_stride, rows, cols, p.accumulate);
                     }
                 }
             }
         }
-        if (STORE != Store::Direct && lane == 0) tc::wait_stores();
+        if (STORE != Store::Direct && lane == 0) tc::wait_store_reads<0>();  // before the shared memory goes
     }
 
     __syncthreads();

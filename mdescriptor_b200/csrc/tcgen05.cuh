@@ -33,16 +33,19 @@ __device__ __forceinline__ void load_tile_pair(void* dst, const CUtensorMap* map
         : "memory");
 }
 
-// 2-D tile store out of shared memory (one bulk group); parts outside the matrix are cut off.
+// 2-D tile store out of shared memory; parts outside the matrix are cut off.
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y, const void* src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
                  "r"(y), "r"(smem_u32(src))
                  : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// Until the stores issued by this thread have read their shared memory / are complete.
-__device__ __forceinline__ void wait_store_reads() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void wait_stores() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Ends a group of this thread's stores; a group may be empty.
+__device__ __forceinline__ void end_stores() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// Until all but the last LEFT groups have read their shared memory.
+template <int LEFT>
+__device__ __forceinline__ void wait_store_reads() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
 
 // ------------------------------------------------------------ clusters
 
