@@ -196,7 +196,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 // moment shows in its block's scale.
 // Bound by HBM (p, m, v in and out, g in) with states of 32 bits; with 8 bits the
 // arithmetic is as long as the traffic: 64 M elements in 211 tensors, float32 p,
-// bfloat16 g, 207 us a step, 4.4 TB/s, 68 % of issue slots used (365 us with exact
+// bfloat16 g, 200 us a step, 4.5 TB/s, 67 % of issue slots used (365 us with exact
 // divisions and codes by conversion).
 template <class P, class G, bool SMALL>
 struct Update {

@@ -45,8 +45,8 @@ struct RowArgs {
 // that also sums s^2, and only the blocks' maxima wait for the row's end (in
 // shared memory, one float a block).  Nothing of the row is held or read twice.
 // Bound by HBM: x and r once in, sum and codes once out.  131 072 x 2100 bfloat16
-// rows with residual: 332 us a pass, 5.8 TB/s (299 us and 1.91 GB of DRAM traffic
-// for the kernel alone, 62 % of issue slots used); with 16-byte units, two blocks
+// rows with residual: 321 us a pass, 6.0 TB/s (302 us and 1.91 GB of DRAM traffic
+// for the kernel alone, 56 % of issue slots used); with 16-byte units, two blocks
 // a warp and the maxima by shuffles it took 593 us, 54 instructions an element.
 template <class T, bool CTA_ROW, Rows MODE>
 struct RowPass {
@@ -282,7 +282,7 @@ void launch_rows(const RowArgs<T>& a, int sms, cudaStream_t stream) {
 // that, so all rows of a CTA are aligned alike and its units are whole 16-byte
 // words of all of them (the first and last of a row partly another row's).
 //
-// 40 001 x 2325 bfloat16 rows with dsum: 159 us a pass, 4.7 TB/s (145 us for this
+// 40 001 x 2325 bfloat16 rows with dsum: 149 us a pass, 5.0 TB/s (142 us for this
 // kernel, 7 for the sum of its partial results); spliced words and no ring took
 // 802 us, aligned words 284, the ring 200.  What is left is its barrier a row.
 template <class T>
@@ -642,8 +642,8 @@ struct TileArgs {
 // TILES: one scale for the whole tile, in both directions.
 // HBM would bound it (every element once in, one byte out a direction), but half
 // of the issue slots' time goes to the arithmetic of two quantisations: 65 536 x
-// 3696 bfloat16 with row factors along columns 166 us, 4.4 TB/s; 32 771 x 1024
-// both ways 37 us, 3.7 TB/s, 57 % of issue slots used.  A persistent form that
+// 3696 bfloat16 with row factors along columns 157 us, 4.7 TB/s; 32 771 x 1024
+// both ways 37 us, 3.7 TB/s, 58 % of issue slots used.  A persistent form that
 // read the next tile ahead took 232 and 55 us: its addresses cost it registers.
 //
 // Two CTAs an SM with both directions of 16-bit elements (37 us for 32 771 x 1024,
