@@ -357,6 +357,43 @@ def test_operators_on_another_stream():
     assert torch.equal(got, want)
 
 
+def test_products_on_two_streams_at_once():
+    """Both streams' kernels want whole SMs and their tensor memory; neither may disturb the other."""
+    a, b = blocks(1, 700, 900)[0], blocks(5, 600, 900, True)[0]
+    few = blocks(9, 5, 900)[0]
+    want, want_few = readout.matmul(a, b), readout.matmul(few, b)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(10):
+        with torch.cuda.stream(streams[0]):
+            got.append((readout.matmul(a, b), want))
+        with torch.cuda.stream(streams[1]):
+            got.append((readout.matmul(few, b), want_few))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in got)
+
+
+def test_products_beyond_32_bit_offsets():
+    # codes: 1 100 000 rows of 4096 bytes
+    codes = torch.randint(0, 256, (1100000, 4096), dtype=torch.uint8, device="cuda", generator=generator(1))
+    codes[(codes & 127) == 127] = 0  # no NaN
+    a = readout.Blocks(codes.view(torch.float8_e4m3fn), torch.rand(1100000, 32, generator=generator(2), device="cuda"))
+    b = blocks(5, 72, 4096, True)[0]
+    got = readout.matmul(a, b, dtype="float32")
+    for rows in (slice(0, 300), slice(1048500, 1048700), slice(1099700, 1100000)):
+        part = readout.Blocks(a.values[rows], a.scales[rows])
+        assert_product(got[rows], part, b)
+    # results: 2.3 G elements, through the copy engine and row by row
+    a, w = blocks(1, 70000, 64)[0], blocks(5, 33000, 64, True)[0]
+    for n in (33000, 32999):
+        b = readout.Blocks(w.values[:n], w.scales)
+        got = readout.matmul(a, b)
+        for rows in (slice(0, 200), slice(69800, 70000)):
+            assert_product(got[rows], readout.Blocks(a.values[rows], a.scales[rows]), b)
+        del got
+
+
 # ---------------------------------------------------------------- optimizer
 
 
