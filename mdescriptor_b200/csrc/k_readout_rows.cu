@@ -668,10 +668,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || (ROWS && !TILES) ? 2 : 3) vo
         a.x.stride * sizeof(T) % sizeof(Word) == 0) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) raw[i] = __ldg(reinterpret_cast<const Word*>(from + i * a.x.stride + col));
-    } else if (tile_row + 128 < rows && tile_col + 128 <= width && (tile_row > 0 || tile_col > 0)) {
+    } else if (tile_row + 128 < rows && (tile_row > 0 || tile_col > 0)) {
         // words of any alignment: something of the matrix lies before and after this tile's part of every row
+        if (col + 4 <= width) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) raw[i] = load_split(from + i * a.x.stride + col);
+            for (int i = 0; i < 16; ++i) raw[i] = load_split(from + i * a.x.stride + col);
+        } else {  // the row ends in or before the quad
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                raw[i] = Word{};
+                T* t = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (col + e < width) t[e] = from[i * a.x.stride + col + e];
+            }
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
