@@ -469,7 +469,7 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         by_type(grad_dtype, [](auto) {});
         if (o.tile_begin.back() == 0) return;
         std::lock_guard<std::mutex> lock(o.mutex);
-        check(cudaSetDevice(o.device), "cudaSetDevice");
+        const OnDevice current(o.device);
         upload(o, static_cast<cudaStream_t>(stream));
         StepSettings a;
         const Tile* tiles = static_cast<const Tile*>(o.table);

@@ -854,7 +854,7 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
                   operand_ok(b, n, b_stride, b_scales, b_tiles && n <= kBlock ? blocks_of(k) : b_scale_stride)),
              "readout: a product's operands need a 16-byte aligned base, a pitch that is a multiple of 16 and a scale "
              "for each block of 128");
-        check(cudaSetDevice(device), "cudaSetDevice");
+        const OnDevice current(device);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         const size_t size = out_dtype == MDSOAP_FLOAT32 ? 4 : 2;
         if (k == 0) {
@@ -876,7 +876,7 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
 
 int mdsoap_matmul_check(int32_t device, void* stream) {
     return entry([&] {
-        check(cudaSetDevice(device), "cudaSetDevice");
+        const OnDevice current(device);
         check(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)), "stream sync");
         unsigned bits = 0;
         check(cudaMemcpyFromSymbol(&bits, g_gave_up, sizeof(bits)), "read product error word");

@@ -643,7 +643,8 @@ struct TileArgs {
 // HBM would bound it (every element once in, one byte out a direction), but half
 // of the issue slots' time goes to the arithmetic of two quantisations: 65 536 x
 // 3696 bfloat16 with row factors along columns 157 us, 4.7 TB/s; 32 771 x 1024
-// both ways 37 us, 3.7 TB/s, 58 % of issue slots used.  A persistent form that
+// both ways 39 us, 3.5 TB/s, 58 % of issue slots used.  Rows that are not aligned
+// to words cost two reads and a splice a quad: 32 427 x 1857 both ways 96 us.  A persistent form that
 // read the next tile ahead took 232 and 55 us: its addresses cost it registers.
 //
 // Two CTAs an SM with both directions of 16-bit elements (37 us for 32 771 x 1024,
@@ -884,7 +885,7 @@ int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride
         if (sum) check_matrix(sum, rows, width, sum_stride, "norm sum");
         if (scales) check_codes(out, rows, width, out_stride, scales, rows, scale_stride, "8-bit rows");
         else check_matrix(out, rows, width, out_stride, "norm output");
-        check(cudaSetDevice(device), "cudaSetDevice");
+        const OnDevice current(device);
         by_type(dtype, [&](auto tag) {
             using T = decltype(tag);
             RowArgs<T> a{};
@@ -934,7 +935,7 @@ int mdsoap_rms_norm_backward(const void* dy, int64_t rows, int64_t width, int64_
         need(width == 0 || (weight && dweight), "readout: the norm gradient needs weight and dweight");
         need(rows == 0 || width == 0 || rstd, "readout: the norm gradient needs rstd");
         if (width == 0) return;
-        check(cudaSetDevice(device), "cudaSetDevice");
+        const OnDevice current(device);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         if (rows == 0) {
             check(cudaMemsetAsync(dweight, 0, width * sizeof(float), s), "clear weight gradient");
@@ -977,7 +978,7 @@ int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride
         if (codes_t)
             check_codes(codes_t, width, rows, code_t_stride, scales_t, tiles ? blocks_of(width) : width,
                         scale_t_stride, "8-bit columns");
-        check(cudaSetDevice(device), "cudaSetDevice");
+        const OnDevice current(device);
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         by_type(dtype, [&](auto tag) {
             using T = decltype(tag);

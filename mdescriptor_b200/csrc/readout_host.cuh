@@ -13,6 +13,21 @@ inline void need(bool ok, const char* message) {
     if (!ok) raise(MDSOAP_INVALID_ARGUMENT, message);
 }
 
+// Makes a device current for the length of a call; the caller's stays what it
+// was (a framework's next allocation goes by it).
+struct OnDevice {
+    int before = 0, now;
+    explicit OnDevice(int device) : now(device) {
+        check(cudaGetDevice(&before), "cudaGetDevice");
+        if (before != now) check(cudaSetDevice(now), "cudaSetDevice");
+    }
+    ~OnDevice() {
+        if (before != now) cudaSetDevice(before);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+};
+
 // Streaming multiprocessors of a device, asked for once.
 inline int sm_count(int device) {
     static std::atomic<int> known[64];
