@@ -293,6 +293,9 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
         const bool vec_a = p.a_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.a_scales) % 16 == 0;
         const bool vec_b = p.b_scale_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.b_scales) % 16 == 0;
         int parity = 0, turn = 0;
+        // The half of b_scale that a turn fills.  It alternates through the whole kernel, from one item to the next
+        // too: the barrier of the turn between lets nobody fill a half that a slower warp still reads.
+        int group = 0;
         for (int item = pair; item < items; item += pairs) {
             const int m0 = item_m(item) + rank * kRows, n0 = item_n(item);
             const int begin = first_block(item), end = last_block(item);
@@ -309,7 +312,7 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
             // four blocks a turn: their scales were loaded one turn ahead
             for (int first = begin & ~3; first < end; first += 4) {
                 float scale[4] = {next_a.x, next_a.y, next_a.z, next_a.w};
-                const int group = first >> 2 & 1;
+                group ^= 1;
                 if constexpr (TILES) {
                     scale[0] *= next_b.x, scale[1] *= next_b.y, scale[2] *= next_b.z, scale[3] *= next_b.w;
                 } else {

@@ -1,0 +1,49 @@
+"""The readout operators where their launches, waits and checks change: many tiles
+for each pair of CTAs, shapes past a limit, other tensors behind an optimizer.
+
+Values are held to the bounds of test_gpu_readout.py.
+"""
+
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from mdescriptor_b200 import readout  # noqa: E402
+from test_gpu_readout import assert_product, blocks, matrix  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _cuda(cuda_device):
+    yield
+
+
+# ---------------------------------------------------------------- products with scales of rows
+
+# 256 tiles (or 120) for 74 pairs of CTAs: each pair goes from tile to tile.  Four blocks of K share a fill of the
+# scales' buffer: 2, 4, 9 and 17 blocks are an odd number of fills, after which the next tile must not take up the
+# same half of it; 1, 5 and 157 an odd or even one beside them.
+MANY_TILES = [(4096, 4096, 128), (4096, 4096, 130), (4096, 4096, 400), (4096, 4096, 520), (4096, 4096, 1100),
+              (4000, 4096, 2100), (3000, 2325, 20000)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_TILES)
+@pytest.mark.parametrize("tiles", [False, True])
+def test_product_of_many_tiles_a_pair(m, n, k, tiles):
+    a, b = blocks(1, m, k)[0], blocks(5, n, k, tiles)[0]
+    for dtype in ("bfloat16", "float32"):
+        got = readout.matmul(a, b, dtype=dtype)
+        assert_product(got, a, b)
+        for _ in range(4):
+            assert torch.equal(got, readout.matmul(a, b, dtype=dtype))
+    # row by row instead of through the copy engine, and added to what is there
+    held = torch.zeros(m, n + 3, device="cuda")
+    out = held[:, 1:1 + n]
+    out.copy_(matrix(9, m, n))
+    before = out.double()
+    readout.matmul(a, b, out=out, accumulate=True)
+    assert_product(out, a, b, before)
+    readout.check()
