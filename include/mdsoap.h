@@ -461,6 +461,12 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
  * or matrix instructions did not complete within their time limit. */
 int mdsoap_matmul_check(int32_t device, void* stream);
 
+/* Failure-detection probe (test support): from now on the first and the second
+ * CTA of each pair copy at most `first` and `second` blocks of K in a product
+ * (every CTA `first` in one of at most 128 rows), so that the matrix
+ * instructions' wait for the next block runs out.  Negative: all, as usual. */
+void mdsoap_probe_matmul(int32_t first, int32_t second);
+
 /* AdamW over many tensors, one launch for every 448 of them:
  *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2  (g times grad_scale);
  *   p = p (1 - lr decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps).

@@ -200,6 +200,8 @@ def _load() -> ctypes.CDLL:
     lib.mdsoap_matmul.argtypes = [_P, i64, i64, _P, i64, _P, i64, i64, _P, i64, i32, i64, i32, i32, _P, i64, _P, i64,
                                   i32, _P]
     lib.mdsoap_matmul_check.argtypes = [i32, _P]
+    lib.mdsoap_probe_matmul.argtypes = [i32, i32]
+    lib.mdsoap_probe_matmul.restype = None
     lib.mdsoap_adamw_create.argtypes = [ctypes.POINTER(AdamWParams), ctypes.POINTER(_P)]
     lib.mdsoap_adamw_step.argtypes = [_P, _P, i32, i64, f64, f64, f64, f64, f64, _P]
     lib.mdsoap_adamw_destroy.argtypes = [_P]
@@ -254,6 +256,7 @@ EXPORTED = (
     "mdsoap_matmul_bytes",
     "mdsoap_matmul",
     "mdsoap_matmul_check",
+    "mdsoap_probe_matmul",
     "mdsoap_adamw_create",
     "mdsoap_adamw_step",
     "mdsoap_adamw_destroy",

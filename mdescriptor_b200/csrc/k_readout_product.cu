@@ -35,6 +35,7 @@ struct ProductArgs {
     int32_t accumulate;
     int32_t splits;   // parts of K, each a work item of its own
     float* partials;  // [split][tile][256][256] where splits > 1
+    int32_t copies[2];  // blocks that the first and the second CTA of a pair copy at most; negative: all (mdsoap_probe_matmul)
 };
 
 // Four neighbouring scales of a row from block `b` on; zero from block `end` on.
@@ -240,13 +241,14 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
     if (warp >= kPromote) {
         tc::give_registers<kFewRegisters>();
         if (warp == kPromote && lane == 0) {
+            const int most = p.copies[rank];
             int stage = 0, phase = 0, count = 0;
             bool good = true;
             for (int item = pair; item < items && good; item += pairs) {
                 const int m0 = item_m(item) + rank * kRows, n0 = item_n(item) + rank * kRows;
                 const int end = last_block(item);
                 for (int kb = first_block(item); kb < end; ++kb, ++count) {
-                    if (!tc::wait(&s.empty[stage], phase ^ 1, gave_up)) {
+                    if (count == most || !tc::wait(&s.empty[stage], phase ^ 1, gave_up)) {
                         good = false;
                         break;
                     }
@@ -367,7 +369,7 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                     turn ^= parity ^ 1;
                 }
             }
-            if (*gave_up) break;
+            if (tc::any_of(1 + half, kRows, *gave_up)) break;  // together: a half's warps meet at barriers
             if constexpr (STORE == Store::Partial && !TILES) {
                 // straight out of the registers: through the copy engine, as below, a part of few blocks ends 4 us
                 // earlier, but this form's loop, short of registers, loses more (1024 x 2100 x 65 537: 281 -> 329 us)
@@ -536,7 +538,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
     if (warp == 4) {
         if (lane == 0) {
             int count = 0;
-            for (int kb = begin; kb < end; ++kb, ++count) {
+            for (int kb = begin; kb < end && count != p.copies[0]; ++kb, ++count) {
                 const int stage = count % kStages;
                 if (!tc::wait(&s.empty[stage], (count / kStages & 1) ^ 1, gave_up)) break;
                 bulk::arrive_expect(&s.full[stage], (kRows + COLS) * kTileK);
@@ -738,6 +740,9 @@ void launch(unsigned grid, unsigned cluster, unsigned threads, size_t bytes, int
     check(cudaLaunchKernelEx(&config, KERNEL, args...), "product launch");
 }
 
+// Blocks that a pair's first and second CTA copy at most (low and high half); the probe's.
+std::atomic<uint64_t> g_copies{~uint64_t(0)};
+
 // What a product of this shape runs.
 struct Shape {
     bool few;
@@ -871,6 +876,9 @@ int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_sca
              "readout: product workspace too small or not 16-byte aligned");
         ProductArgs p{m, n, k, a_scales, a_scale_stride, b_scales, b_scale_stride, b_tiles, out, out_stride, accumulate};
         p.splits = shape.splits;
+        const uint64_t copies = g_copies.load(std::memory_order_relaxed);
+        p.copies[0] = (int32_t)copies;
+        p.copies[1] = (int32_t)(copies >> 32);
         p.partials = static_cast<float*>(workspace);
         if (out_dtype == MDSOAP_FLOAT32) run_product<float>(a, a_stride, b, b_stride, p, shape, sms, device, s);
         else run_product<__nv_bfloat16>(a, a_stride, b, b_stride, p, shape, sms, device, s);
@@ -888,6 +896,10 @@ int mdsoap_matmul_check(int32_t device, void* stream) {
         check(cudaMemcpyToSymbol(g_gave_up, &zero, sizeof(zero)), "clear product error word");
         raise(MDSOAP_INTERNAL, "product: copies or matrix instructions did not complete in time");
     });
+}
+
+void mdsoap_probe_matmul(int32_t first, int32_t second) {
+    g_copies.store((uint64_t)(uint32_t)second << 32 | (uint32_t)first, std::memory_order_relaxed);
 }
 
 }  // extern "C"

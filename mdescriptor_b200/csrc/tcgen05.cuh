@@ -190,7 +190,7 @@ __device__ __forceinline__ void wait_loads() { asm volatile("tcgen05.wait::ld.sy
 // Waits for a barrier phase; false (and *gave_up set) once a second has passed
 // or another thread of the CTA gave up.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* gave_up) {
-    if (bulk::try_wait(bar, parity) || bulk::try_wait(bar, parity)) return true;
+    if (bulk::try_wait(bar, parity) || (!*gave_up && bulk::try_wait(bar, parity))) return true;
     const uint64_t start = bulk::global_ns();
     while (!bulk::try_wait(bar, parity)) {
         if (*gave_up) return false;
@@ -200,6 +200,20 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
         }
     }
     return true;
+}
+
+// Whether `x` is non-zero in any of the `threads` threads that meet at barrier `id`.
+__device__ __forceinline__ bool any_of(int id, int threads, int x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %3, 0;\n\t"
+        "bar.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(threads), "r"(x)
+        : "memory");
+    return r != 0;
 }
 
 // Registers a thread of the calling warpgroup (all four warps): fewer, or more

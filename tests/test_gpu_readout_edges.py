@@ -6,11 +6,14 @@ Values are held to the bounds of test_gpu_readout.py.
 
 from __future__ import annotations
 
+import time
+
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from mdescriptor_b200 import readout  # noqa: E402
+from mdescriptor_b200._lib import lib  # noqa: E402
 from test_gpu_readout import assert_product, blocks, matrix  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -46,4 +49,33 @@ def test_product_of_many_tiles_a_pair(m, n, k, tiles):
     before = out.double()
     readout.matmul(a, b, out=out, accumulate=True)
     assert_product(out, a, b, before)
+    readout.check()
+
+
+# ---------------------------------------------------------------- products whose copies stop
+
+
+@pytest.fixture
+def withheld():
+    """Lets the copies of later products stop after so many blocks; all of them again afterwards."""
+    yield lib.mdsoap_probe_matmul
+    lib.mdsoap_probe_matmul(-1, -1)
+
+
+@pytest.mark.parametrize("m,n,k,tiles,copied", [
+    (700, 600, 1300, False, 3), (700, 600, 1300, True, 0), (1000, 1024, 9000, False, 7), (4096, 4096, 700, False, 8),
+    (4096, 4096, 700, True, 8), (5, 300, 3696, True, 1), (100, 19000, 700, False, 2)])
+def test_product_whose_copies_stop_ends(m, n, k, tiles, copied, withheld):
+    """Each wait ends after its second, the warps that meet at barriers all come to them, and the next product is right."""
+    a, b = blocks(1, m, k)[0], blocks(5, n, k, tiles)[0]
+    readout.check()
+    withheld(copied, copied)
+    start = time.perf_counter()
+    readout.matmul(a, b, dtype="float32")
+    with pytest.raises(RuntimeError, match="did not complete in time"):
+        readout.check()
+    assert time.perf_counter() - start < 8.0  # waits one after the other: a copy, an accumulator, what is in flight
+    readout.check()  # reported once
+    withheld(-1, -1)
+    assert_product(readout.matmul(a, b, dtype="float32"), a, b)
     readout.check()
