@@ -129,10 +129,9 @@ struct PairShared {
     float b_scale[TILES ? 1 : 2][4][TILES ? 4 : kPairTile];
     uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drained;
     uint32_t tensor_memory;
-    int gave_up;
+    int gave_up, other_gave_up;  // this CTA, the pair's other one
     int issued;
 };
-
 
 constexpr int kStep = 16;  // columns that leave tensor memory at a time
 
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
             bulk::barrier_init(&s.acc_empty[i], 2 * kPromote);  // both CTAs' warps
         }
         bulk::barrier_init(&s.drained, 1);
-        s.gave_up = 0;
+        s.gave_up = s.other_gave_up = 0;
         s.issued = 0;
         bulk::barrier_init_fence();
     }
@@ -441,12 +440,23 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
     __syncthreads();
     if (*gave_up && threadIdx.x == 0) {
         atomicOr(&g_gave_up, 1u);
-        // copies in flight land before the shared memory goes
-        if (rank == 0)
-            for (int i = max(0, s.issued - kStages); i < s.issued; ++i)
-                bulk::wait(&s.full[i % kStages], i / kStages & 1);
+        tc::store_shared_at(tc::map_shared(&s.other_gave_up, rank ^ 1), 1);
     }
     tc::cluster_sync();  // neither CTA leaves while the other may still reach into its memory
+    if (*gave_up || *(volatile int*)&s.other_gave_up) {
+        // Both CTAs' copies in flight land before their shared memory goes.  The first CTA's barriers count them, and
+        // it announced both CTAs' bytes for the blocks that it copied; one of the two may have stopped earlier.
+        if (rank == 0 && threadIdx.x == 0) {
+            constexpr uint32_t kEach = 2 * kRows * kTileK;  // bytes of a block that one CTA copies
+            const int mine = s.issued, other = tc::load_int_at(tc::map_shared(&s.issued, 1)), all = max(mine, other);
+            for (int i = min(mine, other); i < all; ++i) {
+                if (mine < other) bulk::arrive_expect(&s.full[i % kStages], kEach);
+                else tc::complete_bytes(&s.full[i % kStages], kEach);
+            }
+            for (int i = max(0, all - kStages); i < all; ++i) bulk::wait(&s.full[i % kStages], i / kStages & 1);
+        }
+        tc::cluster_sync();
+    }
     if (warp == kPromote + 1) tc::dealloc<2>(tmem, 512);
 }
 

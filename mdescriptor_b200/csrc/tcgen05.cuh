@@ -75,6 +75,19 @@ __device__ __forceinline__ float load_shared_at(uint32_t address) {
     return f;
 }
 
+__device__ __forceinline__ int load_int_at(uint32_t address) {
+    int i;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(i) : "r"(address) : "memory");
+    return i;
+}
+__device__ __forceinline__ void store_shared_at(uint32_t address, int value) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(address), "r"(value) : "memory");
+}
+// Counts bytes on a barrier of this CTA that were announced and no copy will bring.
+__device__ __forceinline__ void complete_bytes(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }

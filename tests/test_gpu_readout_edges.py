@@ -79,3 +79,21 @@ def test_product_whose_copies_stop_ends(m, n, k, tiles, copied, withheld):
     withheld(-1, -1)
     assert_product(readout.matmul(a, b, dtype="float32"), a, b)
     readout.check()
+
+
+@pytest.mark.parametrize("first,second", [(5, 3), (3, 5), (0, 2), (2, 0), (7, 6)])
+@pytest.mark.parametrize("tiles", [False, True])
+def test_product_whose_ctas_stop_at_different_blocks(first, second, tiles, withheld):
+    """Neither CTA of a pair leaves before both CTAs' copies have landed, wherever each of them stopped."""
+    a, b = blocks(1, 700, 1300)[0], blocks(5, 600, 1300, tiles)[0]
+    readout.check()
+    withheld(first, second)
+    start = time.perf_counter()
+    readout.matmul(a, b)
+    with pytest.raises(RuntimeError, match="did not complete in time"):
+        readout.check()
+    # a second for the copies that never come, and none for those in flight, which all land
+    assert time.perf_counter() - start < 1.9
+    withheld(-1, -1)
+    assert_product(readout.matmul(a, b), a, b)
+    readout.check()
