@@ -813,7 +813,9 @@ void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
         add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
         check(cudaGetLastError(), "product launch");
     } else if (!p.accumulate && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 &&
-               (p.out_stride * sizeof(OUT)) % 16 == 0) {
+               (p.out_stride * sizeof(OUT)) % 16 == 0 && (p.n * sizeof(OUT)) % 16 == 0) {
+        // the copy engine cuts rows off at whole 16 bytes: in a view whose rows end inside such a piece it would write
+        // over what lies behind them
         const CUtensorMap map_out =
             tile_map(sizeof(OUT) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, sizeof(OUT),
                      p.out, p.m, p.n, p.out_stride, 32);

@@ -33,7 +33,7 @@ __device__ __forceinline__ void load_tile_pair(void* dst, const CUtensorMap* map
         : "memory");
 }
 
-// 2-D tile store out of shared memory; parts outside the matrix are cut off.
+// 2-D tile store out of shared memory; parts outside the matrix are cut off, along a row at whole 16 bytes.
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y, const void* src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x),
                  "r"(y), "r"(smem_u32(src))

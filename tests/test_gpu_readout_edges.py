@@ -97,3 +97,20 @@ def test_product_whose_ctas_stop_at_different_blocks(first, second, tiles, withh
     withheld(-1, -1)
     assert_product(readout.matmul(a, b), a, b)
     readout.check()
+
+
+# ---------------------------------------------------------------- products into views
+
+
+@pytest.mark.parametrize("m,n", [(700, 601), (700, 602), (300, 603), (4000, 4093), (1000, 257), (130, 127), (20, 61)])
+@pytest.mark.parametrize("k", [200, 1300])
+@pytest.mark.parametrize("tiles", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_product_into_a_view_of_whole_pieces(m, n, k, tiles, dtype):
+    """Rows that begin on 16 bytes and end inside such a piece: what lies behind them stays."""
+    a, b = blocks(1, m, k)[0], blocks(5, n, k, tiles)[0]
+    held = torch.full((m + 2, (n // 16 + 2) * 16), 7.0, dtype=dtype, device="cuda")
+    out = held[1:-1, :n]
+    readout.matmul(a, b, out=out)
+    assert_product(out, a, b)
+    assert (held[0] == 7).all() and (held[-1] == 7).all() and (held[:, n:] == 7).all()
