@@ -450,7 +450,9 @@ int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride
  * j' = j / 128 with b_tiles (scales of 128 x 128 tiles), else j.  out is
  * float32 or bfloat16 [m][out_stride]; accumulate != 0 adds to what out holds
  * (float32 only).  `workspace` holds at least mdsoap_matmul_bytes bytes (which
- * may be 0), 16-byte aligned. */
+ * may be 0), 16-byte aligned.  Each wait for a copy or a matrix instruction ends
+ * after a second; results that could not be had are NaN, and
+ * mdsoap_matmul_check reports it. */
 int mdsoap_matmul_bytes(int64_t m, int64_t n, int64_t k, int32_t b_tiles, int32_t device, int64_t* bytes);
 int mdsoap_matmul(const void* a, int64_t m, int64_t a_stride, const float* a_scales, int64_t a_scale_stride,
                   const void* b, int64_t n, int64_t b_stride, const float* b_scales, int64_t b_scale_stride,

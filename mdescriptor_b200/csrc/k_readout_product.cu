@@ -190,6 +190,15 @@ __device__ __forceinline__ void copy_rows(const uint8_t* from, OUT* out, int64_t
     else copy_rows<OUT, BYTES, false>(from, out, stride, rows, cols, add);
 }
 
+// NaN into a warp's 32 rows x kMine columns, of which `rows` and `cols` exist.
+template <class OUT>
+__device__ __forceinline__ void fill_nan(OUT* out, int64_t stride, int64_t rows, int64_t cols) {
+#pragma unroll 1
+    for (int i = 0; i < 32 && i < rows; ++i, out += stride)
+#pragma unroll 1
+        for (int c = threadIdx.x & 31; c < kMine && c < cols; c += 32) out[c] = from_float<OUT>(__int_as_float(-1));
+}
+
 template <bool TILES, class OUT, Store STORE>
 __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_constant__ CUtensorMap map_a,
                                                                    const __grid_constant__ CUtensorMap map_b,
@@ -296,8 +305,8 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
         int parity = 0, turn = 0;
         // The half of b_scale that a turn fills.  It alternates through the whole kernel, from one item to the next
         // too: the barrier of the turn between lets nobody fill a half that a slower warp still reads.
-        int group = 0;
-        for (int item = pair; item < items; item += pairs) {
+        int group = 0, item = pair;
+        for (; item < items; item += pairs) {
             const int m0 = item_m(item) + rank * kRows, n0 = item_n(item);
             const int begin = first_block(item), end = last_block(item);
             const int row = m0 + quarter * 32 + lane, col = n0 + half * kMine;
@@ -433,6 +442,16 @@ __global__ __launch_bounds__(kThreads, 1) void pair_product_kernel(const __grid_
                     }
                 }
             }
+        }
+        // what a half that gave up owes becomes NaN
+#pragma unroll 1
+        for (; item < items; item += pairs) {
+            const int64_t row0 = item_m(item) + rank * kRows + quarter * 32, col0 = item_n(item) + half * kMine;
+            if constexpr (STORE == Store::Partial)
+                fill_nan(p.partials + ((int64_t)item * kPairTile + rank * kRows + quarter * 32) * kPairTile + half * kMine,
+                         kPairTile, 32, kMine);
+            else
+                fill_nan(static_cast<OUT*>(p.out) + row0 * p.out_stride + col0, p.out_stride, p.m - row0, p.n - col0);
         }
         if (STORE != Store::Direct && lane == 0) tc::wait_store_reads<0>();  // before the shared memory goes
     }
@@ -634,9 +653,13 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
                 }
             }
         }
+        if (tc::any_of(1, kRows, *gave_up)) {
+#pragma unroll
+            for (int i = 0; i < COLS / 2; ++i) acc[i] = ~uint64_t(0);  // two NaN
+        }
         if (parts == 1) {
             OUT* q = static_cast<OUT*>(p.out) + n;
-            if (n < p.n && !*gave_up) {
+            if (n < p.n) {
 #pragma unroll
                 for (int i = 0; i < COLS / 2; ++i) {
                     float f[2];
@@ -664,7 +687,7 @@ __global__ __launch_bounds__(kFewThreads, 1) void few_product_kernel(const __gri
     }
     tc::cluster_sync();
     const int64_t n = n0 + threadIdx.x;
-    if (parts > 1 && threadIdx.x < kRows && n < p.n && !*gave_up) {
+    if (parts > 1 && threadIdx.x < kRows && n < p.n) {
         OUT* const out = static_cast<OUT*>(p.out) + n;
         constexpr int kTogether = 8;  // rows whose sums are read at the same time
         for (int j0 = rank; j0 < (int)p.m; j0 += kTogether * parts) {

@@ -270,7 +270,8 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
 
     ``b`` may carry scales of tiles (weights) or of its rows (the weight's
     gradient).  ``dtype`` "bfloat16" or "float32"; ``out`` takes the result, and
-    with ``accumulate`` (float32) has it added."""
+    with ``accumulate`` (float32) has it added.  Results whose copies or matrix
+    instructions did not complete within a second are NaN, and ``check`` raises."""
     m, k, a_ptr, a_stride, a_scale_ptr, a_scale_stride, _ = _blocks(a, "a", False)
     n, k_b, b_ptr, b_stride, b_scale_ptr, b_scale_stride, tiles = _blocks(b, "b", True)
     if k != k_b:

@@ -114,3 +114,24 @@ def test_product_into_a_view_of_whole_pieces(m, n, k, tiles, dtype):
     readout.matmul(a, b, out=out)
     assert_product(out, a, b)
     assert (held[0] == 7).all() and (held[-1] == 7).all() and (held[:, n:] == 7).all()
+
+@pytest.mark.parametrize("m,n,k,tiles,first,second", [
+    (700, 600, 1300, False, 3, 3), (700, 601, 1300, True, 5, 3), (1000, 1024, 9000, False, 7, 8), (300, 300, 2100, True, 2, 2),
+    (4096, 4096, 700, False, 8, 8), (4000, 4096, 700, True, 9, 8), (4000, 4093, 700, True, 8, 8),
+    (5, 300, 3696, True, 1, 1), (100, 700, 1300, False, 2, 2), (60, 19000, 700, False, 2, 2)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_results_that_could_not_be_had_are_nan(m, n, k, tiles, first, second, dtype, withheld):
+    a, b = blocks(1, m, k)[0], blocks(5, n, k, tiles)[0]
+    clean = readout.matmul(a, b, out=torch.zeros(m, n, dtype=dtype, device="cuda"))
+    readout.check()
+    held = torch.full((m + 1, n + 3), 7.0, dtype=dtype, device="cuda")
+    for out in (torch.zeros(m, n, dtype=dtype, device="cuda"), held[1:, :n]):
+        withheld(first, second)
+        readout.matmul(a, b, out=out)
+        with pytest.raises(RuntimeError, match="did not complete in time"):
+            readout.check()
+        withheld(-1, -1)
+        missing = torch.isnan(out)
+        assert missing.any()
+        assert torch.equal(out[~missing], clean[~missing])
+    assert (held[0] == 7).all() and (held[:, n:] == 7).all()
