@@ -484,7 +484,8 @@ template <class OUT>
 __global__ __launch_bounds__(256) void add_parts_kernel(const __grid_constant__ ProductArgs p) {
     const int tiles_n = (int)((p.n + kPairTile - 1) / kPairTile), tiles_m = (int)((p.m + kPairTile - 1) / kPairTile);
     const int64_t part = (int64_t)tiles_n * tiles_m * kPairTile * kPairTile;
-    const int64_t col = (blockIdx.x * 64ll + threadIdx.x % 64) * 4, row = blockIdx.y * 4ll + threadIdx.x / 64;
+    const unsigned across = (unsigned)((p.n + 255) / 256);  // blocks beside one another
+    const int64_t col = (blockIdx.x % across * 64ll + threadIdx.x % 64) * 4, row = blockIdx.x / across * 4ll + threadIdx.x / 64;
     if (row >= p.m || col >= p.n) return;
     const float* from = p.partials + ((row / kPairTile * tiles_n + col / kPairTile) * kPairTile + row % kPairTile) * kPairTile +
                         col % kPairTile;
@@ -832,8 +833,10 @@ void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
         const CUtensorMap map_parts = tile_map(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.partials, s.tiles * s.splits * kPairTile,
                                                kPairTile, kPairTile, 32);
         launch<pair_product_kernel<TILES, float, Store::Partial>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_parts, p);
-        const dim3 add((unsigned)((p.n + 255) / 256), (unsigned)((p.m + 3) / 4));
-        add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
+        // one dimension: the others hold 65 535 blocks, which are 262 140 rows
+        const int64_t add = (p.n + 255) / 256 * ((p.m + 3) / 4);
+        need(add <= 0x7fffffff, "readout: product too large");
+        add_parts_kernel<OUT><<<(unsigned)add, 256, 0, stream>>>(p);
         check(cudaGetLastError(), "product launch");
     } else if (!p.accumulate && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 &&
                (p.out_stride * sizeof(OUT)) % 16 == 0 && (p.n * sizeof(OUT)) % 16 == 0) {

@@ -6,6 +6,7 @@ Values are held to the bounds of test_gpu_readout.py.
 
 from __future__ import annotations
 
+import ctypes
 import time
 
 import pytest
@@ -13,8 +14,8 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from mdescriptor_b200 import readout  # noqa: E402
-from mdescriptor_b200._lib import lib  # noqa: E402
-from test_gpu_readout import assert_product, blocks, matrix  # noqa: E402
+from mdescriptor_b200._lib import lib, raise_for  # noqa: E402
+from test_gpu_readout import assert_product, blocks, generator, matrix  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +51,21 @@ def test_product_of_many_tiles_a_pair(m, n, k, tiles):
     readout.matmul(a, b, out=out, accumulate=True)
     assert_product(out, a, b, before)
     readout.check()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_product_of_many_rows_in_parts(dtype):
+    """Parts of K (one tile more than the pairs take in whole rounds) and more rows than a grid's second dimension holds."""
+    m, n, k = 265472, 250, 40960
+    codes = torch.randint(0, 126, (m, k), dtype=torch.uint8, device="cuda", generator=generator(1))
+    a = readout.Blocks(codes.view(torch.float8_e4m3fn), torch.rand(m, k // 128, generator=generator(2), device="cuda"))
+    b = blocks(5, n, k, True)[0]
+    parts = ctypes.c_int64()
+    raise_for(lib.mdsoap_matmul_bytes(m, n, k, 1, 0, ctypes.byref(parts)))
+    assert parts.value > 0
+    got = readout.matmul(a, b, dtype=dtype)
+    for rows in (slice(0, 300), slice(262100, 262400), slice(m - 300, m)):
+        assert_product(got[rows], readout.Blocks(a.values[rows], a.scales[rows]), b)
 
 
 # ---------------------------------------------------------------- products whose copies stop
