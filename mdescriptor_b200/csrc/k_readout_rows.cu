@@ -239,21 +239,24 @@ __global__ __launch_bounds__(kRowWarps * 32, 4) void rows_kernel(const __grid_co
 }
 
 template <class T, Rows MODE>
-void launch_rows(const RowArgs<T>& a, int sms, cudaStream_t stream) {
+void launch_rows(const RowArgs<T>& a, int device, cudaStream_t stream) {
+    const int sms = sm_count(device);
     if (a.x.rows == 0 || a.x.width == 0) return;
     const int64_t nblocks = blocks_of(a.x.width);
     const bool tops = MODE != Rows::NormWide;
     const size_t warp_bytes = tops ? nblocks * sizeof(float) : 0;
-    if (warp_bytes > 200 * 1024) raise(MDSOAP_INVALID_ARGUMENT, "readout rows: width exceeds 6 553 600 columns");
+    constexpr int kMost = 200 * 1024;
+    if (warp_bytes > kMost) raise(MDSOAP_INVALID_ARGUMENT, "readout rows: width exceeds 6 553 600 columns");
     // A warp a row keeps all reductions inside the warp; a CTA a row when there
     // are too few rows to fill the SMs that way, or the maxima of eight rows
     // would not fit.
     const bool cta_row = a.x.rows < (int64_t)sms * kRowWarps * 2 || warp_bytes * kRowWarps > 48 * 1024;
     if (cta_row) {
         auto kernel = rows_kernel<T, true, MODE>;
-        if (warp_bytes > 48 * 1024)
-            check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)warp_bytes),
-                  "readout rows: shared memory");
+        // the 48 KB that every launch may have hold the kernel's own few bytes too; the limit is the kernel's, not the
+        // launch's, so it is raised once and to the most that any width takes
+        static std::atomic<uint64_t> done;
+        if (warp_bytes > 40 * 1024) allow_shared(kernel, kMost, done, device, "readout rows: shared memory");
         if (a.x.rows > 0x7fffffff) raise(MDSOAP_INVALID_ARGUMENT, "readout rows: too many rows");
         kernel<<<(unsigned)a.x.rows, kRowWarps * 32, warp_bytes, stream>>>(a);
     } else {
@@ -897,17 +900,16 @@ int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride
             a.sum = static_cast<T*>(sum);
             a.sum_stride = sum_stride;
             a.rstd = rstd;
-            const int sms = sm_count(device);
             if (scales) {
                 a.codes = static_cast<uint8_t*>(out);
                 a.code_stride = out_stride;
                 a.scales = scales;
                 a.scale_stride = scale_stride;
-                launch_rows<T, Rows::Norm8>(a, sms, static_cast<cudaStream_t>(stream));
+                launch_rows<T, Rows::Norm8>(a, device, static_cast<cudaStream_t>(stream));
             } else {
                 a.wide = static_cast<T*>(out);
                 a.wide_stride = out_stride;
-                launch_rows<T, Rows::NormWide>(a, sms, static_cast<cudaStream_t>(stream));
+                launch_rows<T, Rows::NormWide>(a, device, static_cast<cudaStream_t>(stream));
             }
         });
     });
@@ -991,7 +993,7 @@ int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride
                 a.code_stride = code_stride;
                 a.scales = scales;
                 a.scale_stride = scale_stride;
-                launch_rows<T, Rows::Quantize>(a, sm_count(device), s);
+                launch_rows<T, Rows::Quantize>(a, device, s);
                 return;
             }
             const TileArgs<T> a{{static_cast<const T*>(x), rows, width, x_stride},

@@ -7,15 +7,16 @@ Values are held to the bounds of test_gpu_readout.py.
 from __future__ import annotations
 
 import ctypes
+import threading
 import time
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from mdescriptor_b200 import readout  # noqa: E402
+from mdescriptor_b200 import _lib, readout  # noqa: E402
 from mdescriptor_b200._lib import lib, raise_for  # noqa: E402
-from test_gpu_readout import assert_product, blocks, generator, matrix  # noqa: E402
+from test_gpu_readout import assert_codes, assert_product, blocks, generator, matrix  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +152,48 @@ def test_results_that_could_not_be_had_are_nan(m, n, k, tiles, first, second, dt
         assert missing.any()
         assert torch.equal(out[~missing], clean[~missing])
     assert (held[0] == 7).all() and (held[:, n:] == 7).all()
+
+
+# ---------------------------------------------------------------- shared memory of wide rows
+
+
+@pytest.mark.parametrize("blocks_", [12279, 12281, 12288, 12289])
+def test_rows_around_the_shared_memory_that_every_launch_has(blocks_):
+    """One float for each block of 128 beside the kernel's own few bytes: 48 KB at 12 280 blocks."""
+    width = blocks_ * 128 - 5
+    x, w = matrix(1, 2, width), torch.ones(width, device="cuda")
+    q = readout.quantize(x).rows
+    assert_codes(q.values, q.scales, x.double())
+    n = readout.rms_norm(x, w, output="float8")
+    assert torch.equal(n.output.values.view(torch.uint8), q.values.view(torch.uint8))
+
+
+def on_two_threads(*calls):
+    """Statuses of calls into the library that run side by side (ctypes lets go of the interpreter's lock)."""
+    seen = []
+
+    def repeat(call):
+        for _ in range(400):
+            seen.append(call())
+
+    threads = [threading.Thread(target=repeat, args=(call,)) for call in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return seen
+
+
+def test_wide_rows_from_two_threads():
+    """Widths that share a kernel and need more shared memory than every launch has, at the same time."""
+    def norm(width):
+        x, w, rstd = torch.ones(1, width, device="cuda"), torch.ones(width, device="cuda"), torch.empty(1, device="cuda")
+        values = torch.empty(1, width, dtype=torch.uint8, device="cuda")
+        scales = torch.empty(1, width // 128, device="cuda")
+        held = (x, w, rstd, values, scales)
+        return lambda: held and lib.mdsoap_rms_norm(
+            x.data_ptr(), 1, width, width, None, 0, _lib.FLOAT32, w.data_ptr(), 1e-6, None, 0, rstd.data_ptr(),
+            values.data_ptr(), width, scales.data_ptr(), width // 128, 0, torch.cuda.current_stream().cuda_stream)
+
+    assert set(on_two_threads(norm(12800 * 128), norm(40000 * 128))) == {_lib.OK}
