@@ -594,15 +594,17 @@ bool alike(const T* p, int64_t stride, const MatrixIn<T>& s) {
 }
 
 template <class T>
-void norm_backward(NormBackwardArgs<T> a, float* dweight, const BackwardShape& s, cudaStream_t stream) {
+void norm_backward(NormBackwardArgs<T> a, float* dweight, const BackwardShape& s, int device, cudaStream_t stream) {
     if (s.threads) {
         const bool same = alike(a.dy.data, a.dy.stride, a.s) && alike(static_cast<const T*>(a.dx), a.dx_stride, a.s) &&
                           (!a.dsum || alike(a.dsum, a.dsum_stride, a.s));
         const auto kernel = s.units == 1   ? (same ? norm_backward_kernel<T, 1, true> : norm_backward_kernel<T, 1, false>)
                             : s.units == 2 ? (same ? norm_backward_kernel<T, 2, true> : norm_backward_kernel<T, 2, false>)
                                            : (same ? norm_backward_kernel<T, 4, true> : norm_backward_kernel<T, 4, false>);
-        const int bytes = ring_depth(s.units) * 3 * s.units * s.threads * 16;  // at most 192 KB
-        check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "norm gradient ring");
+        const int bytes_a_thread = ring_depth(s.units) * 3 * s.units * 16, bytes = bytes_a_thread * s.threads;  // at most 192 KB
+        // raised once to what the widest CTA of this kernel takes: other calls may launch it with other widths meanwhile
+        static std::atomic<uint64_t> done[3][2];
+        allow_shared(kernel, bytes_a_thread * 512, done[s.units / 2][same], device, "norm gradient ring");
         kernel<<<(unsigned)s.grid, s.threads, bytes, stream>>>(a);
     } else {
         a.dots = a.partial + s.grid * s.pitch;
@@ -960,7 +962,7 @@ int mdsoap_rms_norm_backward(const void* dy, int64_t rows, int64_t width, int64_
             a.dx_stride = dx_stride;
             a.partial = static_cast<float*>(workspace);
             a.pitch = shape.pitch;
-            norm_backward<T>(a, dweight, shape, s);
+            norm_backward<T>(a, dweight, shape, device, s);
         });
     });
 }

@@ -197,3 +197,20 @@ def test_wide_rows_from_two_threads():
             values.data_ptr(), width, scales.data_ptr(), width // 128, 0, torch.cuda.current_stream().cuda_stream)
 
     assert set(on_two_threads(norm(12800 * 128), norm(40000 * 128))) == {_lib.OK}
+
+
+def test_norm_gradients_from_two_threads():
+    """Widths that share a kernel and take 48 and 144 KB of its ring, at the same time."""
+    def gradient(width):
+        t = [torch.ones(9, width, device="cuda", dtype=torch.bfloat16) for _ in range(3)]
+        v = [torch.ones(n, device="cuda") for n in (9, width, width)]
+        size = ctypes.c_int64()
+        raise_for(lib.mdsoap_rms_norm_backward_bytes(9, width, _lib.BFLOAT16, 0, ctypes.byref(size)))
+        space = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+        held = (t, v, space)
+        return lambda: held and lib.mdsoap_rms_norm_backward(
+            t[0].data_ptr(), 9, width, width, t[1].data_ptr(), width, v[0].data_ptr(), v[1].data_ptr(), None, 0,
+            _lib.BFLOAT16, t[2].data_ptr(), width, v[2].data_ptr(), space.data_ptr(), size.value, 0,
+            torch.cuda.current_stream().cuda_stream)
+
+    assert set(on_two_threads(gradient(2400), gradient(8000))) == {_lib.OK}
