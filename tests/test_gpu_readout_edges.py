@@ -16,7 +16,7 @@ torch = pytest.importorskip("torch")
 
 from mdescriptor_b200 import _lib, readout  # noqa: E402
 from mdescriptor_b200._lib import lib, raise_for  # noqa: E402
-from test_gpu_readout import assert_codes, assert_product, blocks, generator, matrix  # noqa: E402
+from test_gpu_readout import EPS32, assert_codes, assert_product, blocks, generator, matrix  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -214,3 +214,23 @@ def test_norm_gradients_from_two_threads():
             torch.cuda.current_stream().cuda_stream)
 
     assert set(on_two_threads(gradient(2400), gradient(8000))) == {_lib.OK}
+
+
+# ---------------------------------------------------------------- optimizer
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_adamw_gradients_of_every_size(state_bits):
+    """The first step moves p by lr wherever the gradient's square is a float32, whatever the gradient's size."""
+    sizes = torch.logspace(-18.5, 19, 76, dtype=torch.float64).tolist()
+    params = [torch.zeros(1000, device="cuda") for _ in sizes]
+    grads = [torch.full((1000,), size, device="cuda") for size in sizes]
+    for p, g in zip(params, grads):
+        g[::2].neg_()
+    opt = readout.AdamW(params, lr=1e-3, eps=0.0, weight_decay=0.0, state_bits=state_bits)
+    opt.step(grads)
+    for p, g in zip(params, grads):
+        # v = 0.001 g^2 is off by three roundings, and below the normal range by half of its smallest step too
+        v = 1e-3 * g.double() ** 2
+        slack = 16 * EPS32 + 0.5 * (2.0 ** -150 / v + 2.0 ** -22)
+        assert torch.all((p.double() + 1e-3 * torch.sign(g).double()).abs() <= 1e-3 * slack)
