@@ -23,9 +23,7 @@ One layer y = rms_norm(x + r) W^T and its gradients::
 from __future__ import annotations
 
 import ctypes
-from array import array
 from functools import lru_cache
-from operator import attrgetter
 from typing import NamedTuple, Sequence
 
 import torch
@@ -41,13 +39,13 @@ except ImportError as error:  # no second way: a missing build is an error, as w
 _call.bind(*(ctypes.cast(f, ctypes.c_void_p).value
              for f in (lib.mdsoap_rms_norm, lib.mdsoap_rms_norm_backward, lib.mdsoap_quantize, lib.mdsoap_matmul,
                        lib.mdsoap_adamw_step)))
+_call.use(torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr)
 
 BLOCK = 128
 
 _DTYPES = {torch.float32: _lib.FLOAT32, torch.bfloat16: _lib.BFLOAT16, torch.float16: _lib.FLOAT16}
 _NAMES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 _CODES = torch.float8_e4m3fn
-_dtype_of = attrgetter("dtype")
 
 
 class Blocks(NamedTuple):
@@ -313,13 +311,15 @@ class AdamW:
     """AdamW over all of a readout's tensors in one launch.
 
     ``params``: contiguous CUDA tensors of one type (float32, bfloat16 or
-    float16), updated in place.  ``state_bits`` 32 holds both moments in
+    float16), updated in place, also where one has got other memory since the
+    last step (``p.data = ...``).  ``state_bits`` 32 holds both moments in
     float32; 8 holds them as e4m3 codes with a scale for each 128 elements,
     rounded by dithering with random numbers of (seed, step, element).
     ``weight_decay``: one number, or one a tensor.  ``state``: moments to
     continue from (``exp_avg``, ``exp_avg_sq``, with 8 bits ``exp_avg_scale``
     and ``exp_avg_sq_scale``: lists like ``params``; ``step``: the steps
-    taken), used in place; ``self.state`` has the same form."""
+    taken), used in place; ``self.state`` has the same form.  A tensor of it
+    that is replaced by another one is taken up by the next step."""
 
     def __init__(self, params: Sequence[torch.Tensor], lr: float = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float | Sequence[float] = 0.01, state_bits: int = 32, seed: int = 0,
@@ -330,62 +330,104 @@ class AdamW:
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits = state_bits
-        if not self.params:
+        self._seed = int(seed) & 0xFFFFFFFF
+        count = len(self.params)
+        if not count:
             raise ValueError("AdamW needs at least one tensor")
+        decays = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
+        if len(decays) != count:
+            raise ValueError("weight_decay must be one number or one a tensor")
+        self._decays = decays
+        self._keys = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if state_bits == 8 else 2]
+        self._check_params()
+        if state is None:
+            state = {"step": 0}
+            for key in self._keys:
+                scale = key.endswith("_scale")
+                kind = torch.uint8 if state_bits == 8 and not scale else torch.float32
+                state[key] = [torch.zeros((n + BLOCK - 1) // BLOCK if scale else n, dtype=kind, device=self.device)
+                              for n in self._counts]
+                if kind == torch.uint8:
+                    state[key] = [t.view(_CODES) for t in state[key]]
+        self.state = {"step": int(state["step"]), **{key: list(state[key]) for key in self._keys}}
+        self._bind()
+
+    def _check_params(self) -> None:
         first = self.params[0]
         for p in self.params:
             if not p.is_cuda or not p.is_contiguous() or p.dtype != first.dtype or p.device != first.device:
                 raise ValueError("params must be contiguous CUDA tensors of one type on one device")
-        dtype = _dtype(first, "params")
+        self._dtype = _dtype(first, "params")
         self.device = first.device
+        self._index = first.device.index
         self._counts = [p.numel() for p in self.params]
+
+    def _bind(self) -> None:
+        """Hands the tensors' addresses to the library.
+
+        What it writes to stays alive with it (``_held``): a tensor that is
+        replaced, or given other memory, cannot take the memory away from under
+        a step, and its successor has another address, by which ``step`` sees it."""
+        if len(self.params) != len(self._decays):
+            raise ValueError(f"params must hold {len(self._decays)} tensors")
+        self._check_params()
         count = len(self.params)
-        decays = [float(weight_decay)] * count if isinstance(weight_decay, (int, float)) else [float(w) for w in weight_decay]
-        if len(decays) != count:
-            raise ValueError("weight_decay must be one number or one a tensor")
-        kind = _CODES if state_bits == 8 else torch.float32
         blocks = [(n + BLOCK - 1) // BLOCK for n in self._counts]
-        if state is None:
-            state = {"step": 0}
-            for key in ("exp_avg", "exp_avg_sq"):
-                state[key] = [torch.zeros(n, dtype=torch.uint8, device=self.device).view(_CODES) if state_bits == 8 else
-                              torch.zeros(n, dtype=kind, device=self.device) for n in self._counts]
-                if state_bits == 8:
-                    state[key + "_scale"] = [torch.zeros(n, dtype=torch.float32, device=self.device) for n in blocks]
-        self.state = {"step": int(state["step"])}
         arrays = {"params": self.params}
-        for key in ("exp_avg", "exp_avg_sq"):
-            for name, sizes, want in ((key, self._counts, kind),
-                                      (key + "_scale", blocks, torch.float32))[:2 if state_bits == 8 else 1]:
-                tensors = list(state[name])
-                if len(tensors) != count or any(t.numel() != n or t.dtype != want or t.device != self.device or
-                                                not t.is_contiguous() for t, n in zip(tensors, sizes)):
-                    raise ValueError(f"state {name!r} must hold {count} contiguous {want} tensors that fit the params")
-                self.state[name] = arrays[name] = tensors
+        for key in self._keys:
+            sizes, want = (blocks if key.endswith("_scale") else self._counts,
+                           _CODES if self.state_bits == 8 and not key.endswith("_scale") else torch.float32)
+            tensors = self.state[key]
+            if not isinstance(tensors, list):
+                tensors = self.state[key] = list(tensors)
+            if len(tensors) != count or any(t.numel() != n or t.dtype != want or t.device != self.device or
+                                            not t.is_contiguous() for t, n in zip(tensors, sizes)):
+                raise ValueError(f"state {key!r} must hold {count} contiguous {want} tensors that fit the params")
+            arrays[key] = tensors
         pointers = {key: (ctypes.c_void_p * count)(*[t.data_ptr() for t in v]) for key, v in arrays.items()}
         counts = (ctypes.c_int64 * count)(*self._counts)
-        decay = (ctypes.c_float * count)(*decays)
+        decay = (ctypes.c_float * count)(*self._decays)
         address = {key: ctypes.cast(v, ctypes.c_void_p) for key, v in pointers.items()}
         handle = ctypes.c_void_p()
         raise_for(lib.mdsoap_adamw_create(ctypes.byref(AdamWParams(
             count, address["params"], address["exp_avg"], address["exp_avg_sq"], address.get("exp_avg_scale"),
             address.get("exp_avg_sq_scale"), ctypes.cast(counts, ctypes.c_void_p), ctypes.cast(decay, ctypes.c_void_p),
-            dtype, state_bits, int(seed) & 0xFFFFFFFF, self.device.index)), ctypes.byref(handle)))
+            self._dtype, self.state_bits, self._seed, self._index)), ctypes.byref(handle)))
+        self.close()
         self._optimizer = handle
+        self._held = [t.detach() for v in arrays.values() for t in v]
+        self._param_addresses = _call.addresses(self.params)
+        self._moments = {key: list(arrays[key]) for key in self._keys}
+
+    def _moved(self) -> bool:
+        """Whether a tensor is not the one, or not where, the library writes to."""
+        if _call.addresses(self.params) != self._param_addresses:
+            return True
+        state = self.state
+        for key, held in self._moments.items():
+            if not _call.identical(state[key], held):
+                return True
+        return False
 
     def step(self, grads: Sequence[torch.Tensor], lr: float | None = None, grad_scale: float = 1.0) -> None:
         """Update every tensor with its gradient (one type for all, times ``grad_scale``)."""
-        grads = list(grads)
-        if list(map(torch.Tensor.numel, grads)) != self._counts:
+        if self._moved():
+            self._bind()
+        found = _call.gather(list(grads), self._counts, self._index)
+        if found == 1:
             raise ValueError("grads must be one tensor for each of params, of its size")
-        if (len(set(map(_dtype_of, grads))) != 1 or not all(map(torch.Tensor.is_contiguous, grads))
-                or set(map(torch.Tensor.get_device, grads)) != {self.device.index}):
+        if found == 2:
             raise ValueError(f"grads must be contiguous tensors of one type on {self.device}")
+        pointers, kind = found
+        code = _DTYPES.get(kind)
+        if code is None:
+            raise ValueError(f"grads must be float32, bfloat16 or float16, got {kind}")
         step = self.state["step"] + 1
-        pointers = array("Q", map(torch.Tensor.data_ptr, grads))
-        raise_for(_call.adamw_step(
-            self._optimizer.value, pointers.buffer_info()[0], _dtype(grads[0], "grads"), step, self.lr if lr is None else lr,
-            self.betas[0], self.betas[1], self.eps, grad_scale, _stream(self.device.index)))
+        status = _call.adamw_step(
+            self._optimizer.value, pointers, code, step, self.lr if lr is None else lr,
+            self.betas[0], self.betas[1], self.eps, grad_scale, _stream(self._index))
+        if status:
+            raise_for(status)
         self.state["step"] = step
 
     def close(self) -> None:

@@ -234,3 +234,85 @@ def test_adamw_gradients_of_every_size(state_bits):
         v = 1e-3 * g.double() ** 2
         slack = 16 * EPS32 + 0.5 * (2.0 ** -150 / v + 2.0 ** -22)
         assert torch.all((p.double() + 1e-3 * torch.sign(g).double()).abs() <= 1e-3 * slack)
+
+
+def adamw_pair(state_bits, dtype=torch.float32):
+    """Parameters and gradients of two like optimizers."""
+    sizes = [300, 4097, 5]
+    params = [matrix(i, 1, n, dtype)[0].clone() for i, n in enumerate(sizes)]
+    grads = [matrix(10 + i, 1, n)[0].clone() for i, n in enumerate(sizes)]
+    return params, [p.clone() for p in params], grads
+
+
+def assert_like(a, b):
+    for x, y in zip(a.params, b.params):
+        assert torch.equal(x, y)
+    for key in ("exp_avg", "exp_avg_sq"):
+        for x, y in zip(a.state[key], b.state[key]):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_adamw_takes_up_replaced_state(state_bits):
+    params, others, grads = adamw_pair(state_bits)
+    a, b = readout.AdamW(params, state_bits=state_bits), readout.AdamW(others, state_bits=state_bits)
+    a.step(grads), b.step(grads)
+    saved = {key: value if key == "step" else [t.clone() for t in value] for key, value in a.state.items()}
+    a.step(grads)
+    for x, y in zip(params, others):
+        x.copy_(y)
+    a.state = saved  # back to the first step
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
+    moments = a.state["exp_avg"]
+    moments[2] = moments[2].clone()
+    a.step(grads), b.step(grads)
+    moments[1] = moments[1].clone()
+    a.state["exp_avg_sq"] = tuple(a.state["exp_avg_sq"])
+    before = a.state["exp_avg"][1].view(torch.uint8).clone()
+    junk = [torch.full_like(params[1], 9.0) for _ in range(8)]  # takes memory that nobody holds any more
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
+    assert not torch.equal(a.state["exp_avg"][1].view(torch.uint8), before)
+    assert all((j == 9.0).all() for j in junk)
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+def test_adamw_follows_parameters_to_other_memory(state_bits):
+    params, others, grads = adamw_pair(state_bits)
+    a, b = readout.AdamW(params, state_bits=state_bits), readout.AdamW(others, state_bits=state_bits)
+    a.step(grads), b.step(grads)
+    params[1].data = params[1].data.clone()
+    junk = [torch.full_like(params[1], 9.0) for _ in range(8)]
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
+    a.params[0] = params[0].clone()
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
+    assert all((j == 9.0).all() for j in junk)
+    for p in a.params:
+        p.data = p.data.bfloat16()
+    for p in b.params:
+        p.data = p.data.bfloat16()
+    a.step(grads)
+    again = readout.AdamW(b.params, state_bits=state_bits, state=b.state)
+    again.step(grads)
+    assert_like(a, again)
+
+
+def test_adamw_refuses_replacements_that_do_not_fit():
+    params, _, grads = adamw_pair(32)
+    opt = readout.AdamW(params)
+    opt.step(grads)
+    held = opt.state["exp_avg"][1]
+    opt.state["exp_avg"][1] = held[:-1].clone()
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.step(grads)
+    opt.state["exp_avg"][1] = held
+    params[2].data = torch.ones(9, device="cuda")
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.step(grads)
+    assert opt.state["step"] == 1
+    opt.params.pop()
+    with pytest.raises(ValueError, match="params must hold 3"):
+        opt.step(grads[:2])
