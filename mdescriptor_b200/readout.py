@@ -411,6 +411,8 @@ class AdamW:
 
     def step(self, grads: Sequence[torch.Tensor], lr: float | None = None, grad_scale: float = 1.0) -> None:
         """Update every tensor with its gradient (one type for all, times ``grad_scale``)."""
+        if self._optimizer is None:
+            raise ValueError("the optimizer is closed")
         if self._moved():
             self._bind()
         found = _call.gather(list(grads), self._counts, self._index)
@@ -431,6 +433,7 @@ class AdamW:
         self.state["step"] = step
 
     def close(self) -> None:
+        """Frees the optimizer's table on the device; no step can follow."""
         if self._optimizer:
             lib.mdsoap_adamw_destroy(self._optimizer)
             self._optimizer = None

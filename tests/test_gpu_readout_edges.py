@@ -316,3 +316,14 @@ def test_adamw_refuses_replacements_that_do_not_fit():
     opt.params.pop()
     with pytest.raises(ValueError, match="params must hold 3"):
         opt.step(grads[:2])
+
+
+def test_closed_adamw_refuses_its_step():
+    params, _, grads = adamw_pair(32)
+    opt = readout.AdamW(params)
+    opt.step(grads)
+    opt.close()
+    opt.close()
+    with pytest.raises(ValueError, match="closed"):
+        opt.step(grads)
+    assert opt.state["step"] == 1
