@@ -339,7 +339,7 @@ class AdamW:
             raise ValueError("weight_decay must be one number or one a tensor")
         self._decays = decays
         self._keys = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if state_bits == 8 else 2]
-        self._check_params()
+        self._dtype, self.device, self._counts = self._check_params()
         if state is None:
             state = {"step": 0}
             for key in self._keys:
@@ -352,15 +352,12 @@ class AdamW:
         self.state = {"step": int(state["step"]), **{key: list(state[key]) for key in self._keys}}
         self._bind()
 
-    def _check_params(self) -> None:
+    def _check_params(self) -> tuple[int, torch.device, list[int]]:
         first = self.params[0]
         for p in self.params:
             if not p.is_cuda or not p.is_contiguous() or p.dtype != first.dtype or p.device != first.device:
                 raise ValueError("params must be contiguous CUDA tensors of one type on one device")
-        self._dtype = _dtype(first, "params")
-        self.device = first.device
-        self._index = first.device.index
-        self._counts = [p.numel() for p in self.params]
+        return _dtype(first, "params"), first.device, [p.numel() for p in self.params]
 
     def _bind(self) -> None:
         """Hands the tensors' addresses to the library.
@@ -370,31 +367,32 @@ class AdamW:
         a step, and its successor has another address, by which ``step`` sees it."""
         if len(self.params) != len(self._decays):
             raise ValueError(f"params must hold {len(self._decays)} tensors")
-        self._check_params()
+        dtype, device, numels = self._check_params()
         count = len(self.params)
-        blocks = [(n + BLOCK - 1) // BLOCK for n in self._counts]
+        blocks = [(n + BLOCK - 1) // BLOCK for n in numels]
         arrays = {"params": self.params}
         for key in self._keys:
-            sizes, want = (blocks if key.endswith("_scale") else self._counts,
+            sizes, want = (blocks if key.endswith("_scale") else numels,
                            _CODES if self.state_bits == 8 and not key.endswith("_scale") else torch.float32)
             tensors = self.state[key]
             if not isinstance(tensors, list):
                 tensors = self.state[key] = list(tensors)
-            if len(tensors) != count or any(t.numel() != n or t.dtype != want or t.device != self.device or
+            if len(tensors) != count or any(t.numel() != n or t.dtype != want or t.device != device or
                                             not t.is_contiguous() for t, n in zip(tensors, sizes)):
                 raise ValueError(f"state {key!r} must hold {count} contiguous {want} tensors that fit the params")
             arrays[key] = tensors
         pointers = {key: (ctypes.c_void_p * count)(*[t.data_ptr() for t in v]) for key, v in arrays.items()}
-        counts = (ctypes.c_int64 * count)(*self._counts)
+        counts = (ctypes.c_int64 * count)(*numels)
         decay = (ctypes.c_float * count)(*self._decays)
         address = {key: ctypes.cast(v, ctypes.c_void_p) for key, v in pointers.items()}
         handle = ctypes.c_void_p()
         raise_for(lib.mdsoap_adamw_create(ctypes.byref(AdamWParams(
             count, address["params"], address["exp_avg"], address["exp_avg_sq"], address.get("exp_avg_scale"),
             address.get("exp_avg_sq_scale"), ctypes.cast(counts, ctypes.c_void_p), ctypes.cast(decay, ctypes.c_void_p),
-            self._dtype, self.state_bits, self._seed, self._index)), ctypes.byref(handle)))
+            dtype, self.state_bits, self._seed, device.index)), ctypes.byref(handle)))
         self.close()
         self._optimizer = handle
+        self._dtype, self.device, self._index, self._counts = dtype, device, device.index, numels
         self._held = [t.detach() for v in arrays.values() for t in v]
         self._param_addresses = _call.addresses(self.params)
         self._moments = {key: list(arrays[key]) for key in self._keys}

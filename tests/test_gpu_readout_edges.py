@@ -327,3 +327,19 @@ def test_closed_adamw_refuses_its_step():
     with pytest.raises(ValueError, match="closed"):
         opt.step(grads)
     assert opt.state["step"] == 1
+
+
+def test_adamw_after_a_refused_replacement():
+    """Put back, the refused tensor's predecessor goes on as if nothing had been."""
+    params, others, grads = adamw_pair(32)
+    a, b = readout.AdamW(params), readout.AdamW(others)
+    a.step(grads), b.step(grads)
+    held = params[2].data
+    params[2].data = torch.ones(9, device="cuda")
+    with pytest.raises(ValueError, match="exp_avg"):
+        a.step(grads)
+    params[2].data = held
+    with pytest.raises(ValueError, match="grads"):
+        a.step([*grads[:2], torch.ones(9, device="cuda")])
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
