@@ -412,7 +412,7 @@ int mdsoap_local_compute(const mdsoap_local_params* params, const mdsoap_batch* 
  *   s = x + residual;  rstd = (mean(s^2) + eps)^-1/2;  y = s rstd weight.
  * x, residual (may be NULL), sum (may be NULL; s, for the gradient and the
  * next layer) and a wide y have type `dtype`; rstd (may be NULL) is
- * float32[rows].  With `scales` non-NULL y goes to `out` in 8 bits, else as
+ * float32[rows] (NaN for rows of width 0).  With `scales` non-NULL y goes to `out` in 8 bits, else as
  * `dtype`.  In 8 bits rstd enters the scales alone (it is constant in a row
  * and cancels from the codes), and the rule for tiny blocks looks at s weight. */
 int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride, const void* residual,

@@ -891,6 +891,8 @@ int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride
         if (scales) check_codes(out, rows, width, out_stride, scales, rows, scale_stride, "8-bit rows");
         else check_matrix(out, rows, width, out_stride, "norm output");
         const OnDevice current(device);
+        if (width == 0 && rows > 0 && rstd)  // the mean of no entries: NaN, here from bytes of all ones
+            check(cudaMemsetAsync(rstd, 0xff, rows * sizeof(float), static_cast<cudaStream_t>(stream)), "norm of no columns");
         by_type(dtype, [&](auto tag) {
             using T = decltype(tag);
             RowArgs<T> a{};

@@ -161,7 +161,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | Non
     else:
         out, out_stride, scale_stride = _empty_blocks(rows, width, rows, device)
         out_ptr, scales_ptr = out.values.data_ptr(), out.scales.data_ptr()
-    if rows and width:
+    if rows:
         status = _call.rms_norm(
             x.data_ptr(), rows, width, stride, residual_ptr, residual_stride, dtype, weight_ptr, eps, sum_ptr, width,
             rstd.data_ptr(), out_ptr, out_stride, scales_ptr, scale_stride, index, _stream(index))
@@ -339,7 +339,7 @@ class AdamW:
             raise ValueError("weight_decay must be one number or one a tensor")
         self._decays = decays
         self._keys = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")[:4 if state_bits == 8 else 2]
-        self._dtype, self.device, self._counts = self._check_params()
+        _, self.device, self._counts = self._check_params()
         if state is None:
             state = {"step": 0}
             for key in self._keys:
@@ -392,7 +392,7 @@ class AdamW:
             dtype, self.state_bits, self._seed, device.index)), ctypes.byref(handle)))
         self.close()
         self._optimizer = handle
-        self._dtype, self.device, self._index, self._counts = dtype, device, device.index, numels
+        self.device, self._index, self._counts = device, device.index, numels
         self._held = [t.detach() for v in arrays.values() for t in v]
         self._param_addresses = _call.addresses(self.params)
         self._moments = {key: list(arrays[key]) for key in self._keys}

@@ -216,6 +216,20 @@ def test_norm_gradients_from_two_threads():
     assert set(on_two_threads(gradient(2400), gradient(8000))) == {_lib.OK}
 
 
+@pytest.mark.parametrize("output", [None, "float8"])
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_norm_of_no_columns(output, with_residual):
+    x, w = torch.empty(5, 0, device="cuda"), torch.empty(0, device="cuda")
+    junk = [torch.full((5,), 7.0, device="cuda") for _ in range(8)]
+    del junk  # what a result that nobody fills would hold
+    n = readout.rms_norm(x, w, residual=x if with_residual else None, output=output)
+    assert n.rstd.shape == (5,) and torch.isnan(n.rstd).all()
+    assert n.sum.shape == (5, 0)
+    assert (n.output if output is None else n.output.values).shape == (5, 0)
+    dx, dw = readout.rms_norm_backward(x, n.sum, n.rstd, w)
+    assert dx.shape == (5, 0) and dw.shape == (0,)
+
+
 # ---------------------------------------------------------------- optimizer
 
 
