@@ -886,7 +886,8 @@ int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride
         check_matrix(x, rows, width, x_stride, "norm input");
         check_matrix(residual ? residual : x, rows, width, residual ? residual_stride : x_stride, "norm residual");
         need(weight || width == 0, "readout: the norm needs a weight");
-        need(eps > 0.0 && eps < 1e30, "readout: eps must be positive");
+        // the kernel holds it in float32, where a smaller one is zero: a row of zeros would get an infinite factor
+        need((float)eps > 0.0f && eps < 1e30, "readout: eps must be positive (in float32, too)");
         if (sum) check_matrix(sum, rows, width, sum_stride, "norm sum");
         if (scales) check_codes(out, rows, width, out_stride, scales, rows, scale_stride, "8-bit rows");
         else check_matrix(out, rows, width, out_stride, "norm output");
