@@ -240,8 +240,8 @@ __global__ __launch_bounds__(kRowWarps * 32, 4) void rows_kernel(const __grid_co
 
 template <class T, Rows MODE>
 void launch_rows(const RowArgs<T>& a, int device, cudaStream_t stream) {
-    const int sms = sm_count(device);
     if (a.x.rows == 0 || a.x.width == 0) return;
+    const int sms = sm_count(device);
     const int64_t nblocks = blocks_of(a.x.width);
     const bool tops = MODE != Rows::NormWide;
     const size_t warp_bytes = tops ? nblocks * sizeof(float) : 0;
@@ -863,6 +863,9 @@ void check_matrix(const void* data, int64_t rows, int64_t width, int64_t stride,
     if (!ok) raise(MDSOAP_INVALID_ARGUMENT, std::string("readout: invalid ") + what);
 }
 
+// The row kernel counts columns in 32 bits, past a row's end too.
+constexpr int64_t kWidest = int64_t(1) << 30;
+
 void check_codes(const void* codes, int64_t rows, int64_t width, int64_t stride, const void* scales,
                  int64_t scale_rows, int64_t scale_stride, const char* what) {
     const bool empty = rows == 0 || width == 0;
@@ -885,6 +888,7 @@ int mdsoap_rms_norm(const void* x, int64_t rows, int64_t width, int64_t x_stride
     return entry([&] {
         check_matrix(x, rows, width, x_stride, "norm input");
         check_matrix(residual ? residual : x, rows, width, residual ? residual_stride : x_stride, "norm residual");
+        need(width <= kWidest, "readout: norm input wider than 2^30 columns");
         need(weight || width == 0, "readout: the norm needs a weight");
         // the kernel holds it in float32, where a smaller one is zero: a row of zeros would get an infinite factor
         need((float)eps > 0.0f && eps < 1e30, "readout: eps must be positive (in float32, too)");
