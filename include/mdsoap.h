@@ -494,7 +494,10 @@ typedef struct {
 
 /* Checks and keeps the table of tensors; touches no GPU. */
 int mdsoap_adamw_create(const mdsoap_adamw_params* params, mdsoap_adamw** optimizer);
-/* One step (counted from 1) with the gradients, one a tensor, of grad_dtype. */
+/* One step (counted from 1) with the gradients, one a tensor, of grad_dtype.
+ * Refused on a stream that is being captured: step number, bias corrections and
+ * random numbers would be those of the capture in every replay.  The first step
+ * allocates its table and waits for its upload. */
 int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t grad_dtype, int64_t step, double lr,
                       double beta1, double beta2, double eps, double grad_scale, void* stream);
 void mdsoap_adamw_destroy(mdsoap_adamw* optimizer);

@@ -473,6 +473,10 @@ int mdsoap_adamw_step(mdsoap_adamw* optimizer, const void* const* grads, int32_t
         if (o.tile_begin.back() == 0) return;
         std::lock_guard<std::mutex> lock(o.mutex);
         const OnDevice current(o.device);
+        cudaStreamCaptureStatus capture;
+        check(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture), "optimizer stream");
+        need(capture == cudaStreamCaptureStatusNone,
+             "readout: an optimizer step cannot be captured: every replay would be the same step");
         upload(o, static_cast<cudaStream_t>(stream));
         StepSettings a;
         const Tile* tiles = static_cast<const Tile*>(o.table);

@@ -357,3 +357,23 @@ def test_adamw_after_a_refused_replacement():
         a.step([*grads[:2], torch.ones(9, device="cuda")])
     a.step(grads), b.step(grads)
     assert_like(a, b)
+
+
+@pytest.mark.parametrize("steps_before", [0, 2])
+def test_adamw_refuses_to_be_captured(steps_before):
+    """Replays would repeat one step's number; the first step could not be captured at all."""
+    params, others, grads = adamw_pair(32)
+    a, b = readout.AdamW(params), readout.AdamW(others)
+    for _ in range(steps_before):
+        a.step(grads), b.step(grads)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        doubled = grads[0] * 2.0
+        with pytest.raises(ValueError, match="captured"):
+            a.step(grads)
+    graph.replay()  # what else was captured is whole
+    assert torch.equal(doubled, grads[0] * 2.0)
+    assert a.state["step"] == steps_before
+    a.step(grads), b.step(grads)
+    assert_like(a, b)
