@@ -82,6 +82,10 @@ class Norm(NamedTuple):
     rstd: torch.Tensor
 
 
+# Tells autograd that tensors were written in place, so that a graph that had
+# kept their former values raises an error instead of using these.
+_written = torch.autograd.graph.increment_version
+
 # The handle of a device's current stream, without the Stream object around it.
 _stream = torch._C._cuda_getCurrentRawStream
 
@@ -277,7 +281,8 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
     device, index = a.values.device, a.values.get_device()
     if b.values.get_device() != index:
         raise ValueError("a and b must be on the same device")
-    if out is None:
+    given = out is not None
+    if not given:
         kind = _NAMES.get(dtype)
         if kind is None or kind is torch.float16:
             raise ValueError("dtype must be 'bfloat16' or 'float32'")
@@ -299,6 +304,8 @@ def matmul(a: Blocks, b: Blocks, dtype: str = "bfloat16", out: torch.Tensor | No
         None if workspace is None else workspace.data_ptr(), bytes_, index, _stream(index))
     if status:
         raise_for(status)
+    if given:
+        _written(out)
     return out
 
 
@@ -428,6 +435,7 @@ class AdamW:
             self.betas[0], self.betas[1], self.eps, grad_scale, _stream(self._index))
         if status:
             raise_for(status)
+        _written(self.params)
         self.state["step"] = step
 
     def close(self) -> None:

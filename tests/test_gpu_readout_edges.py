@@ -377,3 +377,23 @@ def test_adamw_refuses_to_be_captured(steps_before):
     assert a.state["step"] == steps_before
     a.step(grads), b.step(grads)
     assert_like(a, b)
+
+
+# ---------------------------------------------------------------- beside autograd
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    """A graph that kept what a call has written over refuses its gradient, as with torch's own in-place operations."""
+    p = torch.nn.Parameter(torch.ones(8, device="cuda"))
+    loss = (p * p).sum()
+    readout.AdamW([p]).step([torch.ones(8, device="cuda")])
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    a, b = blocks(1, 200, 100)[0], blocks(5, 30, 100)[0]
+    for accumulate in (False, True):
+        out = torch.ones(200, 30, device="cuda")
+        x = torch.ones(200, 30, device="cuda", requires_grad=True)
+        loss = (out * x).sum()
+        readout.matmul(a, b, out=out, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
