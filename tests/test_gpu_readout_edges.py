@@ -16,7 +16,8 @@ torch = pytest.importorskip("torch")
 
 from mdescriptor_b200 import _lib, readout  # noqa: E402
 from mdescriptor_b200._lib import lib, raise_for  # noqa: E402
-from test_gpu_readout import EPS32, assert_codes, assert_product, blocks, generator, matrix  # noqa: E402
+from test_gpu_readout import (EPS32, HALF_ULP, assert_codes, assert_product, blocks, generator, matrix, spread, tops,
+                              uniform)  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -377,6 +378,81 @@ def test_adamw_refuses_to_be_captured(steps_before):
     assert a.state["step"] == steps_before
     a.step(grads), b.step(grads)
     assert_like(a, b)
+
+
+# More tiles of 4096 than three CTAs an SM take in two turns, full ones beside partial ones and tensors of no, one and a
+# few elements between them: each CTA goes from tile to tile, reading half a tile ahead where the next one is full.
+MANY_TILES_SIZES = [4096 * 300, 17, 4096 * 200 + 1, 0, 4095, 4096, 1, 4096 * 350 + 129, 300, 4096 * 300, 8192]
+
+
+@pytest.mark.parametrize("state_bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("grad_dtype,offset", [(torch.float32, 0), (torch.bfloat16, 1)])
+def test_adamw_of_many_tiles(state_bits, dtype, grad_dtype, offset):
+    sizes, lr, b1, b2, eps, decay, seed = MANY_TILES_SIZES, 1e-3, 0.9, 0.999, 1e-8, 0.01, 7
+
+    def tensors(like, kind, make):
+        # `offset`: each tensor one element into its memory, so that no unit of four is aligned
+        held = [make(n + offset).to(torch.float32) for n in like]
+        if kind == torch.float8_e4m3fn:
+            return [t.to(torch.uint8).view(kind)[offset:] for t in held]
+        return [t.to(kind)[offset:] for t in held]
+
+    g = generator(3)
+    params = tensors(sizes, dtype, lambda n: 0.1 * torch.randn(n, generator=g, device="cuda"))
+    blocks_ = [(n + 127) // 128 for n in sizes]
+    kind = torch.float8_e4m3fn if state_bits == 8 else torch.float32
+    state = {"step": 0}
+    for key in ("exp_avg", "exp_avg_sq"):
+        state[key] = tensors(sizes, kind, lambda n: torch.zeros(n, device="cuda"))
+        if state_bits == 8:
+            state[key + "_scale"] = tensors(blocks_, torch.float32, lambda n: torch.zeros(n, device="cuda"))
+    opt = readout.AdamW(params, lr=lr, betas=(b1, b2), eps=eps, weight_decay=decay, state_bits=state_bits, seed=seed, state=state)
+    firsts = [sum(blocks_[:i]) * 128 for i in range(len(sizes))]
+    for step in (1, 2):
+        P = [p.double() for p in params]
+        held = {}
+        for key in ("exp_avg", "exp_avg_sq"):
+            held[key] = [t.float().clone() for t in opt.state[key]]
+            if state_bits == 8:
+                held[key] = [t * s.repeat_interleave(128)[:t.numel()] for t, s in zip(held[key], opt.state[key + "_scale"])]
+        grads = tensors(sizes, grad_dtype, lambda n: 0.1 * torch.randn(n, generator=g, device="cuda"))
+        opt.step(grads)
+        noise = uniform(firsts[-1] + sizes[-1], seed, step)
+        for i, n in enumerate(sizes):
+            if n == 0:
+                continue
+            M, V, G = held["exp_avg"][i].double(), held["exp_avg_sq"][i].double(), grads[i].double()
+            m, v = b1 * M + (1 - b1) * G, b2 * V + (1 - b2) * G * G
+            size = b1 * M.abs() + (1 - b1) * G.abs()  # of m's two terms
+            scale = lr / (1 - b1 ** step) / (torch.sqrt(v / (1 - b2 ** step)) + eps)
+            want = P[i] * (1 - lr * decay) - scale * m
+            # m: four roundings of its terms; v's five count half in the root; root, quotient and settings eight more
+            slack = 16 * EPS32 * scale * size + 4 * EPS32 * P[i].abs() + HALF_ULP[dtype] * want.abs()
+            if dtype == torch.float16:
+                slack = slack + 2.0 ** -25  # half of its smallest step
+            assert torch.all((params[i].double() - want).abs() <= slack)
+            if state_bits == 32:
+                assert torch.all((opt.state["exp_avg"][i].double() - m).abs() <= 4 * EPS32 * size)
+                assert torch.all((opt.state["exp_avg_sq"][i].double() - v).abs() <= 5 * EPS32 * v)
+                continue
+            # the states are defined on float32 products (m's two may cancel)
+            m = (held["exp_avg"][i] * b1).double() + (grads[i].float() * (1.0 - b1)).double()
+            for key, x, u in (("exp_avg", m, noise[0]), ("exp_avg_sq", v, noise[1])):
+                top = tops(x.view(1, -1))
+                got_scale = opt.state[key + "_scale"][i].double()
+                assert torch.all((got_scale - top[0] / 448).abs() <= 8 * EPS32 * top[0] / 448)
+                a = 448 * x.abs() / spread(top, n)[0]
+                unit = torch.exp2(torch.floor(torch.log2(a.clamp(min=2.0 ** -6))) - 3)
+                at = a / unit + u[firsts[i]:firsts[i] + n]
+                code = torch.clamp(torch.floor(at) * unit, max=448.0)
+                if key == "exp_avg_sq":
+                    code = torch.where((x > 0) & (code == 0), 2.0 ** -9, code)
+                got = opt.state[key][i].float().double()
+                # a is off by a few float32 roundings of itself (at most 16 steps): 2^-18 of a step, beside u's grid
+                near = (at - torch.round(at)).abs() <= 2.0 ** -17
+                assert torch.all((got.abs() == code) | (near & ((got.abs() - code).abs() <= unit)))
+                assert torch.all((got == 0) | (torch.sign(got) == torch.sign(x)))
 
 
 # ---------------------------------------------------------------- beside autograd
