@@ -484,19 +484,20 @@ template <class OUT>
 __global__ __launch_bounds__(256) void add_parts_kernel(const __grid_constant__ ProductArgs p) {
     const int tiles_n = (int)((p.n + kPairTile - 1) / kPairTile), tiles_m = (int)((p.m + kPairTile - 1) / kPairTile);
     const int64_t part = (int64_t)tiles_n * tiles_m * kPairTile * kPairTile;
-    const unsigned across = (unsigned)((p.n + 255) / 256);  // blocks beside one another
-    const int64_t col = (blockIdx.x % across * 64ll + threadIdx.x % 64) * 4, row = blockIdx.x / across * 4ll + threadIdx.x / 64;
-    if (row >= p.m || col >= p.n) return;
-    const float* from = p.partials + ((row / kPairTile * tiles_n + col / kPairTile) * kPairTile + row % kPairTile) * kPairTile +
-                        col % kPairTile;
-    float4 sum = *reinterpret_cast<const float4*>(from);
+    const int64_t col = (blockIdx.x * 64ll + threadIdx.x % 64) * 4;
+    if (col >= p.n) return;
+    for (int64_t row = blockIdx.y * 4ll + threadIdx.x / 64; row < p.m; row += gridDim.y * 4ll) {
+        const float* from = p.partials + ((row / kPairTile * tiles_n + col / kPairTile) * kPairTile + row % kPairTile) * kPairTile +
+                            col % kPairTile;
+        float4 sum = *reinterpret_cast<const float4*>(from);
 #pragma unroll 4
-    for (int i = 1; i < p.splits; ++i) {
-        const float4 q = *reinterpret_cast<const float4*>(from + i * part);
-        sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+        for (int i = 1; i < p.splits; ++i) {
+            const float4 q = *reinterpret_cast<const float4*>(from + i * part);
+            sum.x += q.x, sum.y += q.y, sum.z += q.z, sum.w += q.w;
+        }
+        const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+        store_row(static_cast<OUT*>(p.out) + row * p.out_stride + col, p.n - col, f, p.accumulate);
     }
-    const float f[4] = {sum.x, sum.y, sum.z, sum.w};
-    store_row(static_cast<OUT*>(p.out) + row * p.out_stride + col, p.n - col, f, p.accumulate);
 }
 
 // ------------------------------------------------------------ few rows
@@ -833,10 +834,9 @@ void run_pairs(const void* a, int64_t a_stride, const void* b, int64_t b_stride,
         const CUtensorMap map_parts = tile_map(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.partials, s.tiles * s.splits * kPairTile,
                                                kPairTile, kPairTile, 32);
         launch<pair_product_kernel<TILES, float, Store::Partial>>(grid, 2, kThreads, bytes, device, stream, map_a, map_b, map_parts, p);
-        // one dimension: the others hold 65 535 blocks, which are 262 140 rows
-        const int64_t add = (p.n + 255) / 256 * ((p.m + 3) / 4);
-        need(add <= 0x7fffffff, "readout: product too large");
-        add_parts_kernel<OUT><<<(unsigned)add, 256, 0, stream>>>(p);
+        // four rows a block; the grid holds 65 535 of them, and taller products go on from there
+        const dim3 add((unsigned)((p.n + 255) / 256), (unsigned)std::min<int64_t>(65535, (p.m + 3) / 4));
+        add_parts_kernel<OUT><<<add, 256, 0, stream>>>(p);
         check(cudaGetLastError(), "product launch");
     } else if (!p.accumulate && reinterpret_cast<uintptr_t>(p.out) % 16 == 0 &&
                (p.out_stride * sizeof(OUT)) % 16 == 0 && (p.n * sizeof(OUT)) % 16 == 0) {
