@@ -395,8 +395,7 @@ int mdsoap_local_compute(const mdsoap_local_params* params, const mdsoap_batch* 
  * the rows).  All pointers are device memory on `device`; matrices are row
  * major with unit column stride and a row pitch ("stride") in elements; work
  * is enqueued on `stream` (a cudaStream_t) and the calls return without
- * waiting and without allocating (the optimizer's first step uploads its
- * table).  Outputs must not overlap inputs unless said.  Sums are held in
+ * waiting and without allocating (but for the optimizer's first step).  Outputs must not overlap inputs unless said.  Sums are held in
  * float32; each stored value is rounded once.
  *
  * 8-bit matrices: e4m3 codes, 16-byte aligned with a pitch that is a multiple
@@ -447,7 +446,8 @@ int mdsoap_quantize(const void* x, int64_t rows, int64_t width, int64_t x_stride
 
 /* Product of two 8-bit matrices along their rows:
  *   out[i][j] = sum_b a_scales[i][b] b_scales[j'][b] sum_{k in block b} a[i][k] b[j][k],
- * j' = j / 128 with b_tiles (scales of 128 x 128 tiles), else j.  out is
+ * j' = j / 128 with b_tiles (scales of 128 x 128 tiles), else j.  The two
+ * scales are multiplied first, in float32.  out is
  * float32 or bfloat16 [m][out_stride]; accumulate != 0 adds to what out holds
  * (float32 only).  `workspace` holds at least mdsoap_matmul_bytes bytes (which
  * may be 0), 16-byte aligned.  Each wait for a copy or a matrix instruction ends

@@ -198,9 +198,9 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[4], const uint32_t (
 // to v more than b2 takes away; a positive v keeps at least the smallest code,
 // since a zero under a non-zero m would make a huge step.  A NaN or infinite
 // moment shows in its block's scale.
-// Bound by HBM (p, m, v in and out, g in) with states of 32 bits; with 8 bits the
-// arithmetic is as long as the traffic: 64 M elements in 211 tensors, float32 p,
-// bfloat16 g, 200 us a step, 4.5 TB/s, 67 % of issue slots used (365 us with exact
+// With 8-bit states neither HBM nor the arithmetic is full: 64 M elements in 211
+// tensors, float32 p, bfloat16 g, 209 us a step (204 to 212 by board), 4.3 TB/s,
+// 70 % of issue slots used by a third of the warps that fit (365 us with exact
 // divisions and codes by conversion).
 template <class P, class G, bool SMALL>
 struct Update {

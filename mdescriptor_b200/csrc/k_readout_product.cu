@@ -96,7 +96,7 @@ __device__ __forceinline__ void store_row(OUT* p, int64_t left, const float (&f)
 // Persistent: the pairs take tiles (and parts of K) in turn, columns first, so
 // that the pairs at work share A's rows and B stays in L2.
 //
-// Measured: 131 072 x 4096 x 3696 into bfloat16 2.41 to 2.45 ms, 1.6 PFLOP/s, with
+// Measured: 131 072 x 4096 x 3696 into bfloat16 2.41 to 2.48 ms, 1.6 PFLOP/s, with
 // the board at its power limit (1.65 GHz at 1000 W); 128 x 128 tiles of one CTA
 // took 3.95 ms.  Two accumulators fill tensor memory, so a block's matrix
 // instructions (512 clocks) wait until its accumulator of two blocks ago has been
@@ -106,7 +106,7 @@ __device__ __forceinline__ void store_row(OUT* p, int64_t left, const float (&f)
 // accumulators of half the columns took 2.7 ms (each instruction reads A again),
 // sixteen warps with half the columns each 2.8 (registers).
 // Scales of B's rows instead of tiles cost a multiplication and a read of shared
-// memory more for every product: 1024 x 2100 x 65 537 into float32 279 us, 1.0
+// memory more for every product: 1024 x 2100 x 65 537 into float32 280 us, 1.0
 // PFLOP/s.
 
 constexpr int kPairTile = 256;

@@ -645,15 +645,17 @@ struct TileArgs {
 // piece ^ column / 4, so that both the stores of a lane's four columns and the
 // reads along a column are free of bank conflicts.
 // TILES: one scale for the whole tile, in both directions.
-// HBM would bound it (every element once in, one byte out a direction), but half
-// of the issue slots' time goes to the arithmetic of two quantisations: 65 536 x
-// 3696 bfloat16 with row factors along columns 157 us, 4.7 TB/s; 32 771 x 1024
-// both ways 39 us, 3.5 TB/s, 58 % of issue slots used.  Rows that are not aligned
+// HBM would bound it (every element once in, one byte out a direction), but a
+// tile's loads and its quantisations follow each other, and the registers leave
+// too few warps (23 % both ways, 35 % along columns) to overlap those of other
+// tiles: 65 536 x 3696 bfloat16 with row factors along columns 157 to 164 us by
+// board, 4.5 to 4.7 TB/s, 56 % of issue slots used; 32 771 x 1024 both ways 39 us,
+// 3.5 TB/s, 57 %.  Rows that are not aligned
 // to words cost two reads and a splice a quad: 32 427 x 1857 both ways 96 us.  A persistent form that
 // read the next tile ahead took 232 and 55 us: its addresses cost it registers.
 //
-// Two CTAs an SM with both directions of 16-bit elements (37 us for 32 771 x 1024,
-// 45 with three, whose 80 registers do not hold the passes), else three, or two
+// Two CTAs an SM with both directions of 16-bit elements (32 771 x 1024 on one
+// board: 37 us, 45 with three, whose 80 registers do not hold the passes), else three, or two
 // for the 64 registers that float32 quads fill.
 template <class T, bool ROWS, bool TILES>
 __global__ __launch_bounds__(256, sizeof(T) == 4 || (ROWS && !TILES) ? 2 : 3) void tile_kernel(const __grid_constant__ TileArgs<T> a) {

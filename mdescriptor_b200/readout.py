@@ -6,7 +6,10 @@ to blocks of 128 (``quantize``, ``matmul``), their gradients
 (``rms_norm_backward``, and ``matmul`` on blocks along columns) and an AdamW
 step over all tensors at once (``AdamW``).  The kernels are those of
 libmdsoap.so; torch tensors hold the memory.  Every call runs on the current
-stream of its tensors' device and returns without waiting.
+stream of its tensors' device and returns without waiting (an optimizer's first
+step, and the one after its tensors changed, makes a table and waits for it).
+Nothing here takes part in autograd: results carry no graph, gradients are calls
+of their own.  Rows are float32, bfloat16 or float16; convert float64 rows first.
 
 One layer y = rms_norm(x + r) W^T and its gradients::
 
